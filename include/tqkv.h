@@ -347,6 +347,114 @@ tqkv_status tqkv_decode_int8_noalloc(const void* q,
                                      cudaStream_t stream);
 
 /* ------------------------------------------------------------------------ */
+/* The KV cache in 4 bits (no counterpart in the reference, whose cache has 8).
+ *
+ * Per row and per block of `block_size` elements, in fp32 with IEEE rounding:
+ *   zero = fp16(min x), scale = fp16((max x - min x) / 15),
+ *   code = round_half_even((x - zero) / scale) clamped to [0, 15], 0 if scale
+ *   is 0; the value read back is code * scale + zero.
+ * A block whose scale or zero is not finite (NaN, an infinity or a value
+ * outside fp16's range in it) is stored as scale = zero = NaN, codes 0: it
+ * reads back as NaN, and attention over it gives NaN.
+ *
+ * Layouts:
+ *   codes  : uint8 [B, H, S_cap, D / 2].  Element i of a row is in 32-bit word
+ *            (i % 32 / 8) * (D / 32) + i / 32, at bits 4 (i % 8) .. + 3
+ *            (little-endian; element 8 l has the lowest bits of its word).
+ *   scales : fp16 [B, H, S_cap, D / block_size, 2] = (scale, zero).
+ * Accepted: D in {64, 128}; block_size in {32, 64, 128}; block_size <= D.
+ * Inputs and outputs are fp16 or bf16 (`dtype`).  Every pointer must be
+ * 16-byte aligned, but starts, lengths and positions (4 bytes).
+ *
+ * `starts` (device, int32 [B]) gives each sequence its own first row; with a
+ * null pointer every sequence's is t0.  With `starts` the rows are known to
+ * the device only: rows outside [0, S_cap) are not written, and read as 0. */
+enum { TQKV_FP16 = 0, TQKV_BF16 = 1 };
+
+/* Quantises x [B, H, T, D] into rows [start, start + T) of a cache.
+ * `x_strides`: the element strides of B, H and T (host array of 3, multiples
+ * of 8; the D elements are adjacent), or null for a contiguous x.  T <= S_cap. */
+tqkv_status tqkv_kv_append_int4(const void* x, const long long* x_strides,
+                                uint8_t* cache_q, void* cache_s,
+                                const int32_t* starts, int t0,
+                                int B, int H, int T, int D, int block_size, int S_cap, int dtype,
+                                cudaStream_t stream);
+
+/* The same for whole contiguous tensors: x [B, H, S, D] into a cache of S rows. */
+tqkv_status tqkv_kv_compress_int4(const void* x, uint8_t* xq, void* scales,
+                                  int B, int H, int S, int D, int block_size, int dtype,
+                                  cudaStream_t stream);
+
+/* y [B, H, T, D] = the values of rows [start, start + T) of a cache. */
+tqkv_status tqkv_kv_reconstruct_int4(const uint8_t* cache_q, const void* cache_s, void* y,
+                                     const int32_t* starts, int t0,
+                                     int B, int H, int T, int D, int block_size, int S_cap,
+                                     int dtype, cudaStream_t stream);
+
+/* Decode attention over a 4-bit cache: q, o [B, H_q, D]; kq, vq and ks, vs as
+ * above with H_kv heads, H_q a multiple of H_kv; query head h attends over K/V
+ * head h / (H_q / H_kv).  Sequence b attends over its first lengths[b] rows
+ * (device, int32 [B]; values are taken into [0, S]), or over S rows if
+ * `lengths` is null; a sequence of no rows gives zeros.  Rows behind the
+ * length are not read.  S <= S_cap only bounds the work split when there are
+ * lengths.
+ * The query heads of a K/V head (up to 8, or 16 in two halves) share one pass
+ * over its rows.  Workspace as for tqkv_decode_int8 (zeroed once by
+ * tqkv_workspace_init, left zeroed by every call, calls that share it
+ * ordered), of tqkv_decode_int4_workspace_bytes; one workspace may serve both.
+ * Results do not depend on scheduling.  Programmatic dependent launches, as
+ * all launches of the 4-bit cache. */
+size_t tqkv_decode_int4_workspace_bytes(int B, int H_q, int H_kv, int S, int D);
+tqkv_status tqkv_decode_int4(const void* q,
+                             const uint8_t* kq, const void* ks,
+                             const uint8_t* vq, const void* vs,
+                             const int32_t* lengths, void* o,
+                             int B, int H_q, int H_kv, int S, int S_cap, int D, int block_size,
+                             int dtype, void* workspace, size_t workspace_bytes,
+                             cudaStream_t stream);
+
+/* Norms of the query and key heads with the position rotation, before the
+ * cache: per head, y = x * rsqrt(mean x^2 + eps) * weight, then for each pair
+ * (a, b) of the first rot_dim elements (a cos - b sin, b cos + a sin); pair j
+ * is elements (j, j + rot_dim / 2), or (2 j, 2 j + 1) if `interleaved`.
+ * Column j of row p of `table` holds (cos, sin) of pair j at position p.
+ * With several axes (time, height, width of an image's tokens) pair j uses
+ * axis 0 for the first sections[0] pairs, axis 1 for the next sections[1], ...
+ * A position outside [0, max_pos) leaves NaN in the token's rotated rows. */
+typedef struct tqkv_norm_rope_args {
+    const void *q, *k;        /* [B, H_q, T, D], [B, H_kv, T, D] with the strides below */
+    const void* v;            /* append: [B, H_kv, T, D] */
+    long long q_strides[3];   /* elements, of B, head and T; multiples of 8 */
+    long long k_strides[3];
+    long long v_strides[3];
+    const void* q_weight;     /* [D], or null for 1 */
+    const void* k_weight;
+    const float* table;       /* [max_pos, rot_dim / 2, 2], 8-byte aligned */
+    const int32_t* positions; /* device, [axes, B, T] */
+    void* q_out;              /* [B, H_q, T, D] */
+    void* k_out;              /* [B, H_kv, T, D]; unused by the append */
+    uint8_t *kq, *vq;         /* append: caches as above */
+    void *ks, *vs;
+    const int32_t* starts;    /* append: first row, as above */
+    double eps;
+    int t0;
+    int B, H_q, H_kv, T, D, block_size, S_cap;
+    int dtype;
+    int rot_dim;              /* a multiple of 16, at most D */
+    int max_pos;
+    int interleaved;
+    int axes;                 /* 1 to 4 */
+    int sections[4];          /* sum rot_dim / 2 if axes > 1 */
+} tqkv_norm_rope_args;
+
+/* q_out and k_out, rounded once to `dtype`. */
+tqkv_status tqkv_qk_norm_rope(const tqkv_norm_rope_args* args, cudaStream_t stream);
+
+/* q_out, and K (normed and rotated, not rounded to `dtype` in between) and V
+ * quantised into rows [start, start + T) of their caches, in one launch. */
+tqkv_status tqkv_qk_norm_rope_append_int4(const tqkv_norm_rope_args* args, cudaStream_t stream);
+
+/* ------------------------------------------------------------------------ */
 /* Device-side failure flag.  Every wait inside the kernels is bounded; a wait
  * that runs out records a nonzero code here (and the kernel returns early)
  * instead of hanging the GPU.  Reads and clears the flag of the current

@@ -1,0 +1,366 @@
+// tqkv_int4.cu — launch planning and C entry points of the 4-bit KV cache:
+// writing, reading back, decode attention, and the head norms with the
+// position rotation (kv_int4.cuh, decode_int4.cuh).
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <atomic>
+#include <climits>
+#include <cmath>
+#include <cstdint>
+
+#include "decode_int4.cuh"
+#include "device_common.cuh"
+#include "kv_int4.cuh"
+#include "launch.h"
+#include "tqkv.h"
+#include "tqkv_internal.h"
+
+namespace tqkv {
+
+// This file's copy of the device error flag (device_common.cuh).
+cudaError_t take_int4_device_error(unsigned int* code) {
+    cudaError_t e = cudaMemcpyFromSymbol(code, g_device_error, sizeof(*code));
+    if (e != cudaSuccess || *code == 0) return e;
+    const unsigned int zero = 0;
+    return cudaMemcpyToSymbol(g_device_error, &zero, sizeof(zero));
+}
+
+namespace {
+
+constexpr int kMaxDevices = 64;
+
+bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+bool is_16bit(int dtype) { return dtype == TQKV_FP16 || dtype == TQKV_BF16; }
+
+// SMs of the current device, looked up once.
+cudaError_t current_sms(int* device, int* sms) {
+    static std::atomic<int> known[kMaxDevices];
+    cudaError_t e = cudaGetDevice(device);
+    if (e != cudaSuccess) return e;
+    if (*device < 0 || *device >= kMaxDevices) return cudaErrorInvalidDevice;
+    int n = known[*device].load(std::memory_order_relaxed);
+    if (n == 0) {
+        e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, *device);
+        if (e != cudaSuccess) return e;
+        known[*device].store(n, std::memory_order_relaxed);
+    }
+    *sms = n;
+    return cudaSuccess;
+}
+
+// Calls f(integral_constant D, integral_constant BS) for an accepted pair.
+template <typename F>
+tqkv_status for_shape(int D, int bs, F&& f) {
+    using std::integral_constant;
+    if (D == 64 && bs == 32) return f(integral_constant<int, 64>{}, integral_constant<int, 32>{});
+    if (D == 64 && bs == 64) return f(integral_constant<int, 64>{}, integral_constant<int, 64>{});
+    if (D == 128 && bs == 32) return f(integral_constant<int, 128>{}, integral_constant<int, 32>{});
+    if (D == 128 && bs == 64) return f(integral_constant<int, 128>{}, integral_constant<int, 64>{});
+    if (D == 128 && bs == 128) return f(integral_constant<int, 128>{}, integral_constant<int, 128>{});
+    return TQKV_ERR_UNSUPPORTED;
+}
+
+// Rows a lane group handles per launch of the write and read kernels.
+template <int D>
+unsigned rows_grid(long long rows) {
+    const long long per = (kInt4Threads / (D / 8)) * static_cast<long long>(kInt4Unroll);
+    return static_cast<unsigned>((rows + per - 1) / per);
+}
+
+tqkv_status make_rows(Int4Rows& g, int B, int H, int T, int D, int S_cap, const int32_t* starts,
+                      int t0) {
+    if (B <= 0 || H <= 0 || T <= 0 || S_cap <= 0 || T > S_cap) return TQKV_ERR_INVALID_SIZE;
+    if (!starts && (t0 < 0 || static_cast<long long>(t0) + T > S_cap)) return TQKV_ERR_INVALID_SIZE;
+    const long long BH = static_cast<long long>(B) * H;
+    if (BH > INT_MAX / T) return TQKV_ERR_INVALID_SIZE;
+    (void)D;
+    g.rows = static_cast<uint32_t>(BH * T);
+    g.T = FastDiv(static_cast<uint32_t>(T));
+    g.H = FastDiv(static_cast<uint32_t>(H));
+    g.S_cap = S_cap;
+    g.starts = starts;
+    g.t0 = t0;
+    g.sb = g.sh = g.st = 0;
+    return TQKV_OK;
+}
+
+bool strides_ok(const long long* s) { return s[0] % 8 == 0 && s[1] % 8 == 0 && s[2] % 8 == 0; }
+
+struct DecodePlan4 {
+    int nt, rec_rows, slices, tile;
+    long long tiles;  // at most: every sequence S rows long
+};
+
+DecodePlan4 plan_int4(int B, int Hq, int Hkv, int S, int D) {
+    DecodePlan4 p{};
+    const int group = Hq / Hkv;
+    p.nt = group > 8 ? 2 : 1;
+    p.rec_rows = group < 8 * p.nt ? group : 8 * p.nt;
+    p.slices = (group + 8 * p.nt - 1) / (8 * p.nt);
+    p.tile = 4096 / D;
+    p.tiles = static_cast<long long>(B) * Hkv * p.slices * ((static_cast<long long>(S) + p.tile - 1) / p.tile);
+    return p;
+}
+
+constexpr int kI4MaxCtasPerSm = 4;  // launch bounds of the decode kernel
+constexpr int kI4MinTiles = kI4Warps;
+
+size_t int4_workspace(const DecodePlan4& p, int D, long long max_ctas) {
+    long long ctas = p.tiles / kI4MinTiles;
+    if (ctas > max_ctas) ctas = max_ctas;
+    if (ctas <= 1) return 0;
+    const size_t counters = (static_cast<size_t>(ctas) * 4 + 255) / 256 * 256;
+    return counters + static_cast<size_t>(ctas) * 2 * p.rec_rows * (D + 4) * sizeof(float);
+}
+
+template <int D, int BS, int NT>
+tqkv_status decode_int4_impl(Int4DecodeArgs a, const DecodePlan4& p, int bf16, void* workspace,
+                             size_t workspace_bytes, cudaStream_t stream) {
+    using C = I4Cfg<D, BS, NT>;
+    int dev = 0, sms = 0;
+    cudaError_t e = current_sms(&dev, &sms);
+    if (e != cudaSuccess) return from_cuda(e);
+    auto fn = decode_int4_kernel<D, BS, NT>;
+    const int smem = C::smem_bytes(p.rec_rows);
+    // opt in and occupancy, once per device and record height
+    static std::atomic<int> known[kMaxDevices][C::kQ + 1];
+    int per_sm = known[dev][p.rec_rows].load(std::memory_order_acquire);
+    if (per_sm == 0) {
+        e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 C::smem_bytes(C::kQ));
+        if (e == cudaSuccess)
+            e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, fn, kI4Threads, smem);
+        if (e != cudaSuccess) return from_cuda(e);
+        if (per_sm < 1) return from_cuda(cudaErrorInvalidConfiguration);
+        if (per_sm > kI4MaxCtasPerSm) per_sm = kI4MaxCtasPerSm;
+        known[dev][p.rec_rows].store(per_sm, std::memory_order_release);
+    }
+    long long grid = p.tiles / kI4MinTiles;
+    if (grid > static_cast<long long>(sms) * per_sm) grid = static_cast<long long>(sms) * per_sm;
+    if (grid < 1) grid = 1;
+    const size_t need = int4_workspace(p, D, static_cast<long long>(sms) * kI4MaxCtasPerSm);
+    if (grid > 1 && (!workspace || workspace_bytes < need)) return TQKV_ERR_WORKSPACE;
+    if (!aligned(workspace, 16)) return TQKV_ERR_MISALIGNED;
+    a.counters = static_cast<unsigned int*>(workspace);
+    a.recs = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) +
+                                      (static_cast<size_t>(grid) * 4 + 255) / 256 * 256);
+    a.min_tiles = kI4MinTiles;
+    return from_cuda(launch_kernel_dependent(fn, dim3(static_cast<unsigned>(grid)),
+                                             dim3(kI4Threads), smem, stream, a, bf16));
+}
+
+}  // namespace
+}  // namespace tqkv
+
+using namespace tqkv;
+
+extern "C" {
+
+tqkv_status tqkv_kv_append_int4(const void* x, const long long* x_strides, uint8_t* cache_q,
+                                void* cache_s, const int32_t* starts, int t0, int B, int H, int T,
+                                int D, int block_size, int S_cap, int dtype, cudaStream_t stream) {
+    if (!is_supported_int8(D, block_size) || !is_16bit(dtype)) return TQKV_ERR_UNSUPPORTED;
+    Int4Rows g;
+    const tqkv_status st = make_rows(g, B, H, T, D, S_cap, starts, t0);
+    if (st != TQKV_OK) return st;
+    if (!x || !cache_q || !cache_s) return TQKV_ERR_NULL;
+    if (!aligned(x, 16) || !aligned(cache_q, 16) || !aligned(cache_s, 16) ||
+        (x_strides && !strides_ok(x_strides)))
+        return TQKV_ERR_MISALIGNED;
+    g.st = x_strides ? x_strides[2] : D;
+    g.sh = x_strides ? x_strides[1] : static_cast<long long>(T) * D;
+    g.sb = x_strides ? x_strides[0] : static_cast<long long>(H) * T * D;
+    return for_shape(D, block_size, [&](auto d, auto bs) {
+        auto fn = dtype == TQKV_BF16 ? kv_append_int4_kernel<d(), bs(), true>
+                                     : kv_append_int4_kernel<d(), bs(), false>;
+        return from_cuda(launch_kernel_dependent(
+            fn, dim3(rows_grid<d()>(g.rows)), dim3(kInt4Threads), 0, stream,
+            static_cast<const uint16_t*>(x), reinterpret_cast<uint32_t*>(cache_q),
+            static_cast<uint32_t*>(cache_s), g));
+    });
+}
+
+tqkv_status tqkv_kv_compress_int4(const void* x, uint8_t* xq, void* scales, int B, int H, int S,
+                                  int D, int block_size, int dtype, cudaStream_t stream) {
+    return tqkv_kv_append_int4(x, nullptr, xq, scales, nullptr, 0, B, H, S, D, block_size, S, dtype,
+                               stream);
+}
+
+tqkv_status tqkv_kv_reconstruct_int4(const uint8_t* cache_q, const void* cache_s, void* y,
+                                     const int32_t* starts, int t0, int B, int H, int T, int D,
+                                     int block_size, int S_cap, int dtype, cudaStream_t stream) {
+    if (!is_supported_int8(D, block_size) || !is_16bit(dtype)) return TQKV_ERR_UNSUPPORTED;
+    Int4Rows g;
+    const tqkv_status st = make_rows(g, B, H, T, D, S_cap, starts, t0);
+    if (st != TQKV_OK) return st;
+    if (!cache_q || !cache_s || !y) return TQKV_ERR_NULL;
+    if (!aligned(cache_q, 16) || !aligned(cache_s, 16) || !aligned(y, 16))
+        return TQKV_ERR_MISALIGNED;
+    return for_shape(D, block_size, [&](auto d, auto bs) {
+        auto fn = dtype == TQKV_BF16 ? kv_reconstruct_int4_kernel<d(), bs(), true>
+                                     : kv_reconstruct_int4_kernel<d(), bs(), false>;
+        return from_cuda(launch_kernel_dependent(
+            fn, dim3(rows_grid<d()>(g.rows)), dim3(kInt4Threads), 0, stream,
+            reinterpret_cast<const uint32_t*>(cache_q), static_cast<const uint32_t*>(cache_s),
+            static_cast<uint4*>(y), g));
+    });
+}
+
+size_t tqkv_decode_int4_workspace_bytes(int B, int H_q, int H_kv, int S, int D) {
+    if (B <= 0 || H_q <= 0 || H_kv <= 0 || H_q % H_kv != 0 || S <= 0 || (D != 64 && D != 128))
+        return 0;
+    int dev = 0, sms = 0;
+    if (current_sms(&dev, &sms) != cudaSuccess) return 0;
+    return int4_workspace(plan_int4(B, H_q, H_kv, S, D), D,
+                          static_cast<long long>(sms) * kI4MaxCtasPerSm);
+}
+
+tqkv_status tqkv_decode_int4(const void* q, const uint8_t* kq, const void* ks, const uint8_t* vq,
+                             const void* vs, const int32_t* lengths, void* o, int B, int H_q,
+                             int H_kv, int S, int S_cap, int D, int block_size, int dtype,
+                             void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+    if (!is_supported_int8(D, block_size) || !is_16bit(dtype)) return TQKV_ERR_UNSUPPORTED;
+    if (B <= 0 || H_q <= 0 || H_kv <= 0 || H_q % H_kv != 0 || S < 0 || S_cap <= 0 || S > S_cap)
+        return TQKV_ERR_INVALID_SIZE;
+    if (static_cast<long long>(B) * H_q > INT_MAX) return TQKV_ERR_INVALID_SIZE;
+    if (!q || !o || !kq || !ks || !vq || !vs) return TQKV_ERR_NULL;
+    if (!aligned(q, 16) || !aligned(o, 16) || !aligned(kq, 16) || !aligned(vq, 16) ||
+        !aligned(ks, 16) || !aligned(vs, 16))
+        return TQKV_ERR_MISALIGNED;
+    Int4DecodeArgs a{};
+    a.q = static_cast<const uint16_t*>(q);
+    a.kq = kq;
+    a.vq = vq;
+    a.ks = static_cast<const uint32_t*>(ks);
+    a.vs = static_cast<const uint32_t*>(vs);
+    a.o = static_cast<uint16_t*>(o);
+    a.lengths = lengths;
+    a.S_cap = S_cap;
+    a.B = B;
+    a.Hq = H_q;
+    a.Hkv = H_kv;
+    a.group = H_q / H_kv;
+    a.S = S;
+    a.score_scale = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(D)));
+    const DecodePlan4 p = plan_int4(B, H_q, H_kv, S, D);
+    a.slices = p.slices;
+    a.rec_rows = p.rec_rows;
+    a.stream_once = 1;
+    const int bf16 = dtype == TQKV_BF16;
+    return for_shape(D, block_size, [&](auto d, auto bs) {
+        return p.nt == 1 ? decode_int4_impl<d(), bs(), 1>(a, p, bf16, workspace, workspace_bytes, stream)
+                         : decode_int4_impl<d(), bs(), 2>(a, p, bf16, workspace, workspace_bytes, stream);
+    });
+}
+
+static tqkv_status rope_checked(const tqkv_norm_rope_args* p, bool append, cudaStream_t stream) {
+    if (!p) return TQKV_ERR_NULL;
+    const int D = p->D, rot = p->rot_dim, axes = p->axes;
+    if ((D != 64 && D != 128) || !is_16bit(p->dtype)) return TQKV_ERR_UNSUPPORTED;
+    if (append && !is_supported_int8(D, p->block_size)) return TQKV_ERR_UNSUPPORTED;
+    if (rot <= 0 || rot > D || rot % 16 != 0 || axes < 1 || axes > 4) return TQKV_ERR_UNSUPPORTED;
+    int sum = 0;
+    for (int i = 0; i < axes; ++i) {
+        if (p->sections[i] < 0) return TQKV_ERR_INVALID_SIZE;
+        sum += p->sections[i];
+    }
+    if (axes > 1 && sum != rot / 2) return TQKV_ERR_INVALID_SIZE;
+    if (p->B <= 0 || p->H_q <= 0 || p->H_kv <= 0 || p->T <= 0 || p->max_pos <= 0)
+        return TQKV_ERR_INVALID_SIZE;
+    if (!(p->eps >= 0.0)) return TQKV_ERR_INVALID_SIZE;
+    const long long tokens = static_cast<long long>(p->B) * p->T;
+    if (tokens > INT_MAX) return TQKV_ERR_INVALID_SIZE;
+    if (append) {
+        if (p->S_cap <= 0 || p->T > p->S_cap) return TQKV_ERR_INVALID_SIZE;
+        if (!p->starts && (p->t0 < 0 || static_cast<long long>(p->t0) + p->T > p->S_cap))
+            return TQKV_ERR_INVALID_SIZE;
+    }
+    if (!p->q || !p->k || !p->q_out || !p->table || !p->positions) return TQKV_ERR_NULL;
+    if (append ? (!p->v || !p->kq || !p->ks || !p->vq || !p->vs) : !p->k_out) return TQKV_ERR_NULL;
+    if (!aligned(p->q, 16) || !aligned(p->k, 16) || !aligned(p->q_out, 16) ||
+        !aligned(p->q_weight, 16) || !aligned(p->k_weight, 16) || !aligned(p->table, 8) ||
+        !strides_ok(p->q_strides) || !strides_ok(p->k_strides))
+        return TQKV_ERR_MISALIGNED;
+    if (append ? (!aligned(p->v, 16) || !strides_ok(p->v_strides) || !aligned(p->kq, 16) ||
+                  !aligned(p->ks, 16) || !aligned(p->vq, 16) || !aligned(p->vs, 16))
+               : !aligned(p->k_out, 16))
+        return TQKV_ERR_MISALIGNED;
+
+    int dev = 0, sms = 0;
+    const cudaError_t e = current_sms(&dev, &sms);
+    if (e != cudaSuccess) return from_cuda(e);
+    RopeArgs a{};
+    a.q = static_cast<const uint16_t*>(p->q);
+    a.k = static_cast<const uint16_t*>(p->k);
+    a.v = static_cast<const uint16_t*>(p->v);
+    a.q_sb = p->q_strides[0], a.q_sh = p->q_strides[1], a.q_st = p->q_strides[2];
+    a.k_sb = p->k_strides[0], a.k_sh = p->k_strides[1], a.k_st = p->k_strides[2];
+    a.v_sb = p->v_strides[0], a.v_sh = p->v_strides[1], a.v_st = p->v_strides[2];
+    a.q_out = static_cast<uint16_t*>(p->q_out);
+    a.k_out = static_cast<uint16_t*>(p->k_out);
+    a.q_w = static_cast<const uint16_t*>(p->q_weight);
+    a.k_w = static_cast<const uint16_t*>(p->k_weight);
+    a.table = reinterpret_cast<const float2*>(p->table);
+    a.pos = p->positions;
+    a.kc = reinterpret_cast<uint32_t*>(p->kq);
+    a.kp = static_cast<uint32_t*>(p->ks);
+    a.vc = reinterpret_cast<uint32_t*>(p->vq);
+    a.vp = static_cast<uint32_t*>(p->vs);
+    a.starts = p->starts;
+    a.eps = p->eps;
+    a.S_cap = p->S_cap;
+    a.tokens = static_cast<uint32_t>(tokens);
+    a.Hq = p->H_q, a.Hkv = p->H_kv, a.T = p->T, a.t0 = p->t0;
+    a.max_pos = p->max_pos, a.rot = rot, a.axes = axes;
+    a.s1 = axes > 1 ? p->sections[0] : INT_MAX;
+    a.s2 = axes > 2 ? a.s1 + p->sections[1] : INT_MAX;
+    a.s3 = axes > 3 ? a.s2 + p->sections[2] : INT_MAX;
+    const int kv_kinds = append ? 2 : 1;
+    const long long rows = tokens * (p->H_q + static_cast<long long>(kv_kinds) * p->H_kv);
+    const int rows_per_cta = kInt4Threads / (D / 8);
+    // one head per lane group while that does not fill the card twice over; then several
+    a.heads_per_group = rows <= 16ll * sms * rows_per_cta ? 1 : 2 * kRopeUnroll;
+    const int hpg = a.heads_per_group;
+    a.q_groups = (p->H_q + hpg - 1) / hpg;
+    a.kv_groups = (p->H_kv + hpg - 1) / hpg;
+    const long long per_token = a.q_groups + static_cast<long long>(kv_kinds) * a.kv_groups;
+    if (per_token * tokens > INT_MAX / 2) return TQKV_ERR_INVALID_SIZE;
+    a.groups = FastDiv(static_cast<uint32_t>(per_token));
+    a.divT = FastDiv(static_cast<uint32_t>(p->T));
+    const unsigned grid = static_cast<unsigned>((per_token * tokens + rows_per_cta - 1) / rows_per_cta);
+    const bool bf16 = p->dtype == TQKV_BF16, inter = p->interleaved != 0;
+    auto launch = [&](auto fn) {
+        return from_cuda(launch_kernel_dependent(fn, dim3(grid), dim3(kInt4Threads), 0, stream, a));
+    };
+    if (!append) {
+        if (D == 64)
+            return bf16 ? (inter ? launch(qk_norm_rope_kernel<64, 32, true, false, true>)
+                                 : launch(qk_norm_rope_kernel<64, 32, true, false, false>))
+                        : (inter ? launch(qk_norm_rope_kernel<64, 32, false, false, true>)
+                                 : launch(qk_norm_rope_kernel<64, 32, false, false, false>));
+        return bf16 ? (inter ? launch(qk_norm_rope_kernel<128, 32, true, false, true>)
+                             : launch(qk_norm_rope_kernel<128, 32, true, false, false>))
+                    : (inter ? launch(qk_norm_rope_kernel<128, 32, false, false, true>)
+                             : launch(qk_norm_rope_kernel<128, 32, false, false, false>));
+    }
+    return for_shape(D, p->block_size, [&](auto d, auto bs) {
+        return bf16 ? (inter ? launch(qk_norm_rope_kernel<d(), bs(), true, true, true>)
+                             : launch(qk_norm_rope_kernel<d(), bs(), true, true, false>))
+                    : (inter ? launch(qk_norm_rope_kernel<d(), bs(), false, true, true>)
+                             : launch(qk_norm_rope_kernel<d(), bs(), false, true, false>));
+    });
+}
+
+tqkv_status tqkv_qk_norm_rope(const tqkv_norm_rope_args* args, cudaStream_t stream) {
+    return rope_checked(args, false, stream);
+}
+
+tqkv_status tqkv_qk_norm_rope_append_int4(const tqkv_norm_rope_args* args, cudaStream_t stream) {
+    return rope_checked(args, true, stream);
+}
+
+}  // extern "C"

@@ -24,6 +24,22 @@ STATUS_NAMES = {
     6: "TQKV_ERR_NULL",
 }
 
+class NormRopeArgs(ctypes.Structure):
+    """tqkv_norm_rope_args of include/tqkv.h."""
+    _fields_ = [
+        ("q", c_void_p), ("k", c_void_p), ("v", c_void_p),
+        ("q_strides", ctypes.c_longlong * 3), ("k_strides", ctypes.c_longlong * 3),
+        ("v_strides", ctypes.c_longlong * 3),
+        ("q_weight", c_void_p), ("k_weight", c_void_p), ("table", c_void_p),
+        ("positions", c_void_p), ("q_out", c_void_p), ("k_out", c_void_p),
+        ("kq", c_void_p), ("vq", c_void_p), ("ks", c_void_p), ("vs", c_void_p),
+        ("starts", c_void_p), ("eps", ctypes.c_double), ("t0", c_int),
+        ("B", c_int), ("H_q", c_int), ("H_kv", c_int), ("T", c_int), ("D", c_int),
+        ("block_size", c_int), ("S_cap", c_int), ("dtype", c_int), ("rot_dim", c_int),
+        ("max_pos", c_int), ("interleaved", c_int), ("axes", c_int), ("sections", c_int * 4),
+    ]
+
+
 # C ABI: name -> (restype, argtypes)
 C_ABI = {
     "tqkv_status_string": (ctypes.c_char_p, [c_int]),
@@ -74,6 +90,14 @@ C_ABI = {
     "tqkv_decode_int8_append_exchange": (c_int, [c_void_p] * 8 + [c_int] * 7 +
                                          [c_void_p, c_size_t, ctypes.POINTER(c_void_p), c_int,
                                           c_int, c_void_p]),
+    "tqkv_kv_append_int4": (c_int, [c_void_p, ctypes.POINTER(ctypes.c_longlong)] + [c_void_p] * 3 +
+                            [c_int] * 8 + [c_void_p]),
+    "tqkv_kv_compress_int4": (c_int, [c_void_p] * 3 + [c_int] * 6 + [c_void_p]),
+    "tqkv_kv_reconstruct_int4": (c_int, [c_void_p] * 4 + [c_int] * 8 + [c_void_p]),
+    "tqkv_decode_int4_workspace_bytes": (c_size_t, [c_int] * 5),
+    "tqkv_decode_int4": (c_int, [c_void_p] * 7 + [c_int] * 8 + [c_void_p, c_size_t, c_void_p]),
+    "tqkv_qk_norm_rope": (c_int, [ctypes.POINTER(NormRopeArgs), c_void_p]),
+    "tqkv_qk_norm_rope_append_int4": (c_int, [ctypes.POINTER(NormRopeArgs), c_void_p]),
 }
 
 # The reference's C++ launchers (include/attention.h, include/quantization.h),

@@ -1,0 +1,252 @@
+"""Decode attention over the 4-bit cache (tqkv_decode_int4), against attention over the cache's
+values in float64."""
+import numpy as np
+import pytest
+import torch
+
+import tqkv
+from tqkv import Workspace
+
+from int4_reference import VALID, check_attention
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+def _rand(shape, seed, dtype=F16):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(shape, generator=g, device="cuda").to(dtype)
+
+
+def _cache(B, H, S, D, bs, seed, mul=1.0):
+    return tqkv.kv_compress_int4(_rand((B, H, S, D), seed) * mul, bs)
+
+
+def _run(B, Hq, Hkv, S, D, bs, dtype=F16, lengths=None, seed=0, **kw):
+    q = _rand((B, Hq, D), seed + 1, dtype)
+    kq, ks = _cache(B, Hkv, S, D, bs, seed + 2)
+    vq, vs = _cache(B, Hkv, S, D, bs, seed + 3)
+    n = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    o = tqkv.decode_int4(q, kq, ks, vq, vs, bs, lengths=n, **kw)
+    assert tqkv.read_device_error() == 0
+    return o, q, kq, ks, vq, vs
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("D,bs", VALID)
+@pytest.mark.parametrize("S", [1, 2, 15, 16, 17, 31, 32, 33, 64, 65, 127, 129, 500])
+def test_lengths_around_the_tiles(S, D, bs, dtype):
+    o, q, *cache = _run(2, 3, 3, S, D, bs, dtype, seed=S)
+    check_attention(o, q, *cache, bs, [S, S])
+
+
+@pytest.mark.parametrize("D,bs", VALID)
+@pytest.mark.parametrize("Hq,Hkv", [(1, 1), (2, 1), (6, 2), (5, 1), (8, 1), (9, 1), (16, 1), (24, 2),
+                                    (17, 1), (40, 1), (33, 3)])
+def test_groups_of_query_heads(Hq, Hkv, D, bs):
+    o, q, *cache = _run(2, Hq, Hkv, 333, D, bs, seed=Hq)
+    check_attention(o, q, *cache, bs, [333, 333])
+
+
+@pytest.mark.parametrize("D,bs,G", [(128, 128, 1), (128, 32, 4), (64, 32, 16), (64, 64, 7)])
+@pytest.mark.parametrize("S", [9000, 20011])
+def test_heads_cut_across_many_blocks(S, D, bs, G):
+    o, q, *cache = _run(1, G, 1, S, D, bs, BF16, seed=S + G)
+    check_attention(o, q, *cache, bs, [S])
+
+
+@pytest.mark.parametrize("D,bs,G", [(128, 64, 4), (64, 32, 1), (128, 32, 12)])
+def test_ragged_lengths(D, bs, G):
+    S = 700
+    lengths = [700, 0, 1, 33, 0, 699, 256, 64, 0, 5, 128, 31] + list(range(40, 75))
+    o, q, *cache = _run(len(lengths), 2 * G, 2, S, D, bs, lengths=lengths, seed=G)
+    check_attention(o, q, *cache, bs, lengths)
+    for b, n in enumerate(lengths):
+        if n == 0:
+            assert not o[b].any()
+
+
+def test_lengths_are_taken_into_the_range():
+    lengths = [-5, 2 ** 31 - 1, -2 ** 31, 41]
+    _, q, *cache = _run(4, 2, 1, 100, 128, 64)
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    o = tqkv.decode_int4(q, *cache, 64, S=40, lengths=n)
+    check_attention(o, q, *cache, 64, [0, 40, 0, 40])
+
+
+def test_all_sequences_empty():
+    q = _rand((3, 4, 64), 1)
+    cache = [t for n in (2, 3) for t in _cache(3, 2, 50, 64, 32, n)]
+    out = torch.full_like(q, 9.0)
+    tqkv.decode_int4(q, *cache, 32, lengths=torch.zeros(3, dtype=torch.int32, device="cuda"), out=out)
+    assert not out.any()
+    out.fill_(9.0)
+    tqkv.decode_int4(q, *cache, 32, S=0, out=out)
+    assert not out.any()
+
+
+@pytest.mark.parametrize("D,bs", VALID)
+def test_rows_behind_the_length_are_not_read(D, bs):
+    """NaN and arbitrary bytes behind each length change nothing, and the caches stay as they are."""
+    B, Hq, Hkv, S = 3, 4, 2, 150
+    lengths = [1, 70, 149]
+    o, q, kq, ks, vq, vs = _run(B, Hq, Hkv, S, D, bs, lengths=lengths)
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    for b, m in enumerate(lengths):
+        kq[b, :, m:], vq[b, :, m:] = 0xFF, 0xFF
+        ks[b, :, m:], vs[b, :, m:] = float("nan"), float("inf")
+    before = [t.clone() for t in (kq, ks, vq, vs)]
+    again = tqkv.decode_int4(q, kq, ks, vq, vs, bs, lengths=n)
+    assert torch.equal(o, again)
+    for t, u in zip((kq, ks, vq, vs), before):
+        assert torch.equal(t.view(torch.uint8), u.view(torch.uint8))
+
+
+def test_nan_reaches_only_its_head():
+    o, q, kq, ks, vq, vs = _run(2, 4, 2, 100, 128, 32)
+    ks[1, 0, 50, 2] = float("nan")
+    vs[0, 1, 7, 1] = float("nan")
+    again = tqkv.decode_int4(q, kq, ks, vq, vs, 32)
+    assert torch.isnan(again[1, :2]).all()
+    assert torch.isnan(again[0, 2:, 32:64]).all() and not torch.isnan(again[0, 2:, :32]).any()
+    assert torch.equal(again[0, :2], o[0, :2]) and torch.equal(again[1, 2:], o[1, 2:])
+
+
+@pytest.mark.parametrize("kmul,vmul,qmul", [(1, 1e-4, 1), (1, 2e4, 1), (30, 1, 1), (1e-3, 1, 1e3),
+                                            (1, 1, 0), (200, 1e3, 0.5), (1, 1, 1e-6)])
+@pytest.mark.parametrize("D,bs", [(128, 32), (64, 64)])
+def test_magnitudes(D, bs, kmul, vmul, qmul):
+    """Weights and values of every magnitude, peaked and flat scores."""
+    B, Hq, Hkv, S = 1, 4, 2, 400
+    q = (_rand((B, Hq, D), 1).float() * qmul).half()
+    kq, ks = _cache(B, Hkv, S, D, bs, 2, kmul)
+    vq, vs = tqkv.kv_compress_int4((_rand((B, Hkv, S, D), 3).float().clamp(-2.5, 2.5) * vmul).half(), bs)
+    o = tqkv.decode_int4(q, kq, ks, vq, vs, bs)
+    check_attention(o, q, kq, ks, vq, vs, bs, [S])
+
+
+def test_one_token_far_above_many_small_ones():
+    """A token of a large weight and a small value scale beside thousands of small weights whose
+    values are large: their sum must not be lost below fp16's range."""
+    S, D, bs = 8000, 128, 128
+    q = torch.zeros((1, 1, D), dtype=F16, device="cuda")
+    q[..., 0] = 10.0
+    k = _rand((1, 1, S, D), 4) * 0.01
+    k[0, 0, 4321, 0] = 14.0
+    v = _rand((1, 1, S, D), 5) * 30 + 20
+    v[0, 0, 4321] *= 1e-4
+    kq, ks = tqkv.kv_compress_int4(k, bs)
+    vq, vs = tqkv.kv_compress_int4(v, bs)
+    o = tqkv.decode_int4(q, kq, ks, vq, vs, bs)
+    check_attention(o, q, kq, ks, vq, vs, bs, [S])
+
+
+def test_bf16_queries_beyond_fp16():
+    q = (_rand((1, 2, 128), 1).float() * 1e5).to(BF16)
+    assert float(q.abs().max()) > 65504
+    kq, ks = _cache(1, 2, 77, 128, 64, 2, 1e-4)
+    vq, vs = _cache(1, 2, 77, 128, 64, 3)
+    o = tqkv.decode_int4(q, kq, ks, vq, vs, 64)
+    check_attention(o, q, kq, ks, vq, vs, 64, [77])
+
+
+def test_offsets_past_32_bits():
+    D, bs, S_cap = 128, 128, 1 << 25
+    codes = [torch.empty((1, 3, S_cap, D // 2), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    scales = [torch.empty((1, 3, S_cap, 1, 2), dtype=F16, device="cuda") for _ in range(2)]
+    n = 130
+    for i in range(2):
+        tqkv.kv_append_int4(_rand((1, 3, n, D), i), codes[i], scales[i], 0, bs)
+    q = _rand((1, 3, D), 5)
+    o = tqkv.decode_int4(q, codes[0], scales[0], codes[1], scales[1], bs, S=n)
+    small = [t[:, :, :n].contiguous() for p in zip(codes, scales) for t in p]
+    assert torch.equal(o, tqkv.decode_int4(q, *small, bs))
+    check_attention(o, q, *small, bs, [n])
+
+
+def test_results_repeat_and_the_workspace_is_left_zeroed():
+    B, Hq, Hkv, S, D, bs = 3, 8, 2, 5000, 128, 64
+    lengths = [5000, 17, 3333]
+    o, q, *cache = _run(B, Hq, Hkv, S, D, bs, lengths=lengths)
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    ws = Workspace()
+    for _ in range(20):
+        assert torch.equal(o, tqkv.decode_int4(q, *cache, bs, lengths=n, workspace=ws))
+    assert not ws.buf.any()
+
+
+def test_workspace_shared_with_the_int8_decode():
+    ws = Workspace()
+    B, H, S, D, bs = 1, 4, 30000, 128, 64
+    q, k, v = _rand((B, H, D), 1), _rand((B, H, S, D), 2), _rand((B, H, S, D), 3)
+    c8 = [*tqkv.kv_compress(k, bs), *tqkv.kv_compress(v, bs)]
+    c4 = [*tqkv.kv_compress_int4(k, bs), *tqkv.kv_compress_int4(v, bs)]
+    o8, o4 = tqkv.decode_int8(q, *c8, bs), tqkv.decode_int4(q, *c4, bs)
+    for _ in range(3):
+        assert torch.equal(o8, tqkv.decode_int8(q, *c8, bs, workspace=ws))
+        assert torch.equal(o4, tqkv.decode_int4(q, *c4, bs, workspace=ws))
+
+
+def test_streams_side_by_side():
+    """Calls on several streams at once, each with the workspace of its stream."""
+    sets = []
+    for i in range(3):
+        q = _rand((1, 8, 128), 10 * i)
+        sets.append((q, *_cache(1, 2, 9000, 128, 64, 10 * i + 1), *_cache(1, 2, 9000, 128, 64, 10 * i + 2)))
+    want = [tqkv.decode_int4(*s, 64) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(10):
+        got = [tqkv.decode_int4(*s, 64, stream=st) for s, st in zip(sets, streams)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_graphs_captured_on_one_stream_replay_side_by_side():
+    """Two captured calls own their scratch: replays on different streams do not disturb each
+    other, and lengths may change between replays."""
+    sets, graphs, outs, lens = [], [], [], []
+    for i in range(2):
+        q = _rand((2, 8, 128), 10 * i)
+        sets.append((q, *_cache(2, 2, 6000, 128, 64, 10 * i + 1), *_cache(2, 2, 6000, 128, 64, 10 * i + 2)))
+        lens.append(torch.tensor([6000, 100], dtype=torch.int32, device="cuda"))
+    for s, n in zip(sets, lens):
+        tqkv.decode_int4(*s, 64, lengths=n)
+    torch.cuda.synchronize()
+    for s, n in zip(sets, lens):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(tqkv.decode_int4(*s, 64, lengths=n))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in sets]
+    for lengths in ([6000, 100], [1, 5999], [0, 3000]):
+        for n in lens:
+            n.copy_(torch.tensor(lengths))
+        want = [tqkv.decode_int4(*s, 64, lengths=n) for s, n in zip(sets, lens)]
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for g, st in zip(graphs, streams):
+                with torch.cuda.stream(st):
+                    g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def test_workspace_does_not_grow_while_captured():
+    q = _rand((1, 8, 128), 1)
+    cache = (*_cache(1, 2, 6000, 128, 64, 2), *_cache(1, 2, 6000, 128, 64, 3))
+    ws = Workspace()
+    tqkv.decode_int4(q, *cache, 64)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with pytest.raises(ValueError, match="captured"):
+            tqkv.decode_int4(q, *cache, 64, workspace=ws)
+    want = tqkv.decode_int4(q, *cache, 64, workspace=ws)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = tqkv.decode_int4(q, *cache, 64, workspace=ws)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
