@@ -26,25 +26,35 @@
 // error 2^-12 a token, like the 16-bit P of any tensor-core attention).  The
 // zero sums stay in fp32.
 //
-// Range.  p * scale must stay inside fp16 whatever the caches hold, so the
-// running reference of the softmax is M >= max_t(score_t + log2 of the scale's
-// upper power of two), in base 2, and the operand is 2^(score - M + 11) *
-// scale < 2^11; M moves only when a token exceeds it by 2^4.
+// V's codes enter as code - 8 (one packed fp16 subtraction, exact) beside zero
+// + 8 scale: sums of codes 0..15 would grow with the length while O does not,
+// and what the tensor core cuts off each sum, and p's rounding, would grow
+// with them.  K's zero terms are a product as well: a column of zeros times
+// the blocks' sums of q in two fp16 words.
+//
+// Range.  p * scale must stay inside fp16 whatever the caches hold: the
+// operand is 2^(score - M - e + 11) * scale with M within 2^4 of the largest
+// score so far and 2^e above the largest scale, so it is below 2^15, and
+// tokens 2^-25 of the largest keep all their bits.
 //
 // Work split.  Units are (sequence, KV head, slice of 8 * NT query heads); a
-// unit has ceil(length / TILE) tiles.  All units' tiles, end to end, are cut
-// into equal runs, one per CTA, whatever the lengths are; the CTA's 4 warps
-// take its tiles in turn.  A unit that lies in one CTA is finished there; of a
-// unit cut across CTAs each leaves a record (acc[D], M, l per query head) in
-// the workspace, and the CTA that arrives last at the unit's counter merges
-// the records in order: the result does not depend on which one that is.
-// Records and counters are zeroed again by the CTA that merges.
+// unit has ceil(length / 16) granules.  All units' granules, end to end, are cut
+// into equal runs, one per CTA, and each CTA's run into equal runs, one per
+// warp, whatever the lengths are.  A warp meets at most one unit that began
+// before its run and one that goes on behind it; units that lie within its run
+// it finishes alone, without meeting another warp.  The states (acc[D], l, its
+// reference, per query head) of cut units are joined in order: within the CTA
+// in shared memory at the end of the run, across CTAs through records in the
+// workspace, by the CTA that arrives last at the unit's counter.  The order
+// does not depend on which one that is.  The merging CTA zeroes the records
+// and the counter again.
 //
-// Every warp streams for itself: a ring of STAGES tiles, K and V rows by bulk
-// copies (one lane), the parameters by one cp.async per row, which fills rows
-// behind the sequence's end with zeros: their codes are whatever the buffer
-// held (any 4 bits are finite), their weights are zero, and rows past the
-// length are never read.
+// Every warp streams for itself: a ring of STAGES tiles filled by cp.async (16
+// bytes a lane, past L1), waited for by group, with no barrier between warps.
+// Rows behind the sequence's end are filled with zeros and are not read.
+// 16-byte chunks are exchanged within a row so that both ways the tile is read
+// (a row's chunks side by side for K, one chunk of every second row for V) are
+// free of bank conflicts.
 #pragma once
 
 #include <cstdint>
@@ -56,8 +66,11 @@
 
 namespace tqkv {
 
-constexpr int kI4Warps = 4;
-constexpr int kI4Threads = kI4Warps * 32;
+constexpr int kGranule = 16;     // rows by which runs are cut
+// Resident warps: 12 leave each 168 registers (16 of 128 spill, and 8 hide less
+// latency: B1 H32 S65536 at block size 128 takes 54.4 us with 12, 63.3 with 16
+// and 59.7 with 8); two tiles of accumulators (NT = 2) need 8.
+constexpr int kI4MaxWarps = 12;
 
 struct Int4DecodeArgs {
     const uint16_t* q;          // [B, Hq, D]
@@ -70,9 +83,15 @@ struct Int4DecodeArgs {
     long long S_cap;
     int B, Hq, Hkv, group, slices, S;
     int rec_rows;               // query heads a record holds: min(group, 8 * NT)
-    int min_tiles;              // tiles a CTA takes at least
-    int stream_once;            // L2: the cache will not be read again soon
+    int stages;                 // ring stages a warp has: 2 or 3
     float score_scale;          // log2(e) / sqrt(D)
+};
+
+// A unit that a warp's run cuts: its first granule (-1: none, -2: the warp has
+// no run), the one behind its last, its first output row b * Hq + h, and its
+// query heads.
+struct alignas(16) CutUnit {
+    int start, end, row, nq;
 };
 
 template <int D, int BS, int NT>
@@ -81,17 +100,25 @@ struct I4Cfg {
     static constexpr int kSub = D / 32;           // 32-element groups = words per lane chunk
     static constexpr int kNS = D / BS;            // blocks a row
     static constexpr int kTile = 4096 / D;        // rows a tile: 2 KB of codes
-    static constexpr int kM = kTile / 16;         // 16-row pieces
+    static constexpr int kM = kTile / 16;         // granules a tile
     static constexpr int kQ = 8 * NT;             // query heads a unit takes
     static constexpr int kKV = kTile * kRow;
     static constexpr int kSc = kTile * kNS * 4;
     static constexpr int kStage = 2 * (kKV + kSc);
-    static constexpr int kStages = 3;
-    static constexpr int kRing = kI4Warps * kStages * kStage;
-    static constexpr int kRecStride = D + 4;      // acc[D], l at D, M at D + 1
-    static constexpr int kOffMerge = kRing + kI4Warps * kStages * 8 + 16;
-    static_assert(kOffMerge % 16 == 0, "alignment");
-    static int smem_bytes(int rows) { return kOffMerge + kI4Warps * rows * kRecStride * 4; }
+    static constexpr int kRecStride = D + 4;      // acc[D], l at D, R at D + 1
+    static constexpr int kWarps = NT == 1 ? kI4MaxWarps : 8;  // an SM's
+    // bytes of the states of `rows` query heads
+    __host__ __device__ static constexpr int state(int rows) { return rows * kRecStride * 4; }
+    // a warp's ring: it takes the state of the unit that goes on behind its run
+    // once all its tiles are used
+    __host__ __device__ static constexpr int ring(int stages, int rows) {
+        return stages * kStage > state(rows) ? stages * kStage : state(rows);
+    }
+    // rings, the states of the units that began before a run, two descriptors a
+    // warp, flags
+    static int smem_bytes(int warps, int stages, int rows) {
+        return warps * (ring(stages, rows) + state(rows) + 2 * static_cast<int>(sizeof(CutUnit))) + 16;
+    }
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
@@ -100,6 +127,15 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
         "{%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// (code - 8) * 2^-U of the codes in the low (U = 24) or next (20) nibbles
+template <int U>
+__device__ __forceinline__ uint32_t minus8(uint32_t x) {
+    const uint32_t code = x & (U == 24 ? 0x000f000fu : 0x00f000f0u);
+    const __half2 eight = __half2half2(__ushort_as_half(U == 24 ? 0x0008 : 0x0080));
+    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&code), eight);
+    return *reinterpret_cast<const uint32_t*>(&v);
 }
 
 // transpose of an 8 x 8 matrix of 16-bit values held two to a lane
@@ -111,24 +147,28 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
 
 // `bytes` (4, 8 or 16) of global memory into shared memory, or zeros
 template <int bytes>
-__device__ __forceinline__ void cp_async_zfill(uint32_t dst, const void* src, bool real) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(bytes),
-                 "r"(real ? bytes : 0)
-                 : "memory");
+__device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool real = true) {
+    if constexpr (bytes == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+                     "r"(real ? 16 : 0)
+                     : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src),
+                     "n"(bytes), "r"(real ? bytes : 0)
+                     : "memory");
 }
-__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar))
-                 : "memory");
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// bulk copy without an L2 hint
-__device__ __forceinline__ void bulk_copy_g2s_plain(void* dst, const void* src, uint32_t bytes,
-                                                    uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-            smem_addr(dst)),
-        "l"(src), "r"(bytes), "r"(smem_addr(bar))
-        : "memory");
+// N words from shared memory by one load
+template <int N>
+__device__ __forceinline__ void lds_words(uint32_t (&w)[N], const uint8_t* p) {
+    if constexpr (N == 4) *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(p);
+    else if constexpr (N == 2) *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(p);
+    else w[0] = *reinterpret_cast<const uint32_t*>(p);
 }
 
 __device__ __forceinline__ int i4_length(const Int4DecodeArgs& a, int b) {
@@ -137,19 +177,47 @@ __device__ __forceinline__ int i4_length(const Int4DecodeArgs& a, int b) {
     return n < 0 ? 0 : n > a.S ? a.S : n;
 }
 
-// The unit that a tile belongs to, moved forward tile by tile.
-template <int TILE>
+// Arrives at a counter: everything that this CTA wrote before the barrier in
+// front of it is visible to whoever sees the counter's new value.
+__device__ __forceinline__ unsigned int arrive_acq_rel(unsigned int* p) {
+    unsigned int before;
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(p) : "memory");
+    return before;
+}
+
+// Four elements of an output row.
+__device__ __forceinline__ void store_out(uint16_t* dst, float4 v, int bf16) {
+    uint2 out;
+    out.x = bf16 ? pack2<true>(v.x, v.y) : pack2<false>(v.x, v.y);
+    out.y = bf16 ? pack2<true>(v.z, v.w) : pack2<false>(v.z, v.w);
+    *reinterpret_cast<uint2*>(dst) = out;
+}
+
+// (v, lr) += (x, xr): sums and their l relative to 2^reference; empty states
+// have l = 0 at -infinity.
+__device__ __forceinline__ void join(float4& v, float2& lr, float4 x, float2 xr) {
+    const float m = fmaxf(lr.y, xr.y);
+    const float f = lr.y == m ? 1.0f : fast_exp2(lr.y - m);
+    const float e = xr.y == m ? 1.0f : fast_exp2(xr.y - m);
+    v.x = fmaf(x.x, e, v.x * f);
+    v.y = fmaf(x.y, e, v.y * f);
+    v.z = fmaf(x.z, e, v.z * f);
+    v.w = fmaf(x.w, e, v.w * f);
+    lr = make_float2(fmaf(xr.x, e, lr.x * f), m);
+}
+
+// The unit that a granule belongs to, moved forward.
 struct UnitWalk {
-    int b, u;         // sequence; (KV head, slice) within it
-    int len, nt;      // its rows and tiles
-    long long start;  // first tile of the unit
+    int b, u;     // sequence; (KV head, slice) within it
+    int len, nt;  // its rows and granules
+    int start;    // first granule of the unit
 
     __device__ __forceinline__ void load(const Int4DecodeArgs& a) {
         len = b < a.B ? i4_length(a, b) : 0;
-        nt = (len + TILE - 1) / TILE;
+        nt = (len + kGranule - 1) / kGranule;
     }
     // g below the total: the loop ends
-    __device__ __forceinline__ void seek(const Int4DecodeArgs& a, long long g) {
+    __device__ __forceinline__ void seek(const Int4DecodeArgs& a, int g) {
         while (g >= start + nt && b < a.B) {
             start += nt;
             if (nt > 0 && ++u < a.Hkv * a.slices) continue;
@@ -161,155 +229,219 @@ struct UnitWalk {
 };
 
 template <int D, int BS, int NT>
-__global__ void __launch_bounds__(kI4Threads, NT == 1 ? 4 : 2)
-    decode_int4_kernel(Int4DecodeArgs a, int bf16) {
+__global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
+    decode_int4_kernel(const Int4DecodeArgs a, int bf16) {
     using C = I4Cfg<D, BS, NT>;
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int nw = blockDim.x >> 5;
     const int g = lane >> 2, c = lane & 3;  // the mma's row and column groups
-    uint8_t* ring = smem + warp * C::kStages * C::kStage;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kRing) + warp * C::kStages;
-    unsigned int* flag = reinterpret_cast<unsigned int*>(smem + C::kRing + kI4Warps * C::kStages * 8);
-    float* merge = reinterpret_cast<float*>(smem + C::kOffMerge);
-
-    if (lane == 0) {
-        for (int i = 0; i < C::kStages; ++i) mbar_init(bars + i, 33);  // 32 lanes' parameters, 1 codes
-        fence_barrier_init();
-    }
-    __syncwarp();
+    const int rows = a.rec_rows;
+    const int ring_bytes = C::ring(a.stages, rows);
+    const int state_floats = rows * C::kRecStride;
+    uint8_t* ring = smem + warp * ring_bytes;
+    float* merge = reinterpret_cast<float*>(smem + nw * ring_bytes);  // [warp] state
+    CutUnit* cuts = reinterpret_cast<CutUnit*>(merge + nw * state_floats);  // [warp][2]
+    unsigned int* flags = reinterpret_cast<unsigned int*>(cuts + 2 * nw);   // [2]
     griddep_wait();
     griddep_launch_dependents();
 
-    // ---- this CTA's tiles [g0, g1) of all units' n
+    // ---- this CTA's granules [g0, g1) of all units' n: n / ctas each, one more for
+    // the first n % ctas CTAs
     const int per_seq = a.Hkv * a.slices;
-    long long n = 0;
+    int n = 0, of_lane = 0;  // of sequence `lane`
+    bool empty = false;
     if (a.lengths == nullptr) {
-        n = static_cast<long long>(a.B) * per_seq * ((a.S + C::kTile - 1) / C::kTile);
+        n = a.B * ((a.S + kGranule - 1) / kGranule);
+        empty = a.S == 0;
     } else {
-        for (int b = lane; b < a.B; b += 32) n += (i4_length(a, b) + C::kTile - 1) / C::kTile;
+        for (int b = lane; b < a.B; b += 32) {
+            const int len = i4_length(a, b);
+            const int x = (len + kGranule - 1) / kGranule;
+            if (b == lane) of_lane = x;
+            n += x;
+            empty |= len == 0;
+        }
 #pragma unroll
         for (int off = 16; off; off >>= 1) n += __shfl_xor_sync(0xffffffffu, n, off);
-        n *= per_seq;
+        empty = __any_sync(0xffffffffu, empty);
     }
-    // heads of sequences that hold nothing come out as zero
-    if (a.lengths != nullptr || a.S == 0) {
+    n *= per_seq;
+    if (empty) {  // heads of sequences that hold nothing come out as zero
         for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
             if (i4_length(a, b) != 0) continue;
             uint32_t* o = reinterpret_cast<uint32_t*>(a.o) + static_cast<long long>(b) * a.Hq * (D / 2);
-            for (int i = threadIdx.x; i < a.Hq * (D / 2); i += kI4Threads) o[i] = 0u;
+            for (int i = threadIdx.x; i < a.Hq * (D / 2); i += blockDim.x) o[i] = 0u;
         }
     }
-    long long ctas = n / a.min_tiles;
-    if (ctas > gridDim.x) ctas = gridDim.x;
-    if (ctas < 1) ctas = 1;
-    const long long cta = blockIdx.x;
+    // at least a tile for every warp of a CTA that works
+    unsigned ctas = static_cast<unsigned>(n) / (nw * C::kM);
+    ctas = ctas > gridDim.x ? gridDim.x : ctas < 1 ? 1 : ctas;
+    const unsigned cta = blockIdx.x;
     if (cta >= ctas || n == 0) return;
-    const long long g0 = n * cta / ctas, g1 = n * (cta + 1) / ctas;
-    auto cta_of = [&](long long tile) { return ((tile + 1) * ctas - 1) / n; };
-
-    UnitWalk<C::kTile> walk;  // of the unit being worked on
-    if (a.lengths == nullptr) {
-        const int nt = (a.S + C::kTile - 1) / C::kTile;
-        const long long unit = g0 / nt;
-        walk.b = static_cast<int>(unit / per_seq);
-        walk.u = static_cast<int>(unit - static_cast<long long>(walk.b) * per_seq);
-        walk.start = unit * nt;
-        walk.load(a);
-    } else {
-        walk.start = 0;
-        walk.b = 0;
-        for (int base = 0; base < a.B; base += 32) {
-            const int b = base + lane;
-            long long x = b < a.B ? static_cast<long long>((i4_length(a, b) + C::kTile - 1) / C::kTile) * per_seq
-                                  : 0;
-#pragma unroll
-            for (int off = 1; off < 32; off <<= 1) {
-                const long long y = __shfl_up_sync(0xffffffffu, x, off);
-                if (lane >= off) x += y;
-            }
-            const unsigned past = __ballot_sync(0xffffffffu, walk.start + x <= g0);
-            const int k = __popc(past);  // sequences of these 32 that end at or before g0
-            if (k > 0) {
-                walk.start += __shfl_sync(0xffffffffu, x, k - 1);
-                walk.b = base + k;
-            }
-            if (k < 32) break;
-        }
-        walk.load(a);
-        const long long in = g0 - walk.start;
-        walk.u = static_cast<int>(in / walk.nt);
-        walk.start += static_cast<long long>(walk.u) * walk.nt;
-    }
-
-    // ---- this warp's stream of tiles: g0 + warp, g0 + warp + 4, ...
-    const uint64_t policy = make_evict_first_policy();
-    UnitWalk<C::kTile> ahead = walk;
-    long long next = g0 + warp;
-    int issued = 0;
-    auto issue = [&]() {
-        if (next >= g1) return;
-        ahead.seek(a, next);
-        const int st = issued % C::kStages;
-        uint8_t* buf = ring + st * C::kStage;
-        uint64_t* bar = bars + st;
-        const int t0 = static_cast<int>(next - ahead.start) * C::kTile;
-        const int rows = ahead.len - t0 < C::kTile ? ahead.len - t0 : C::kTile;
-        const int h = ahead.u / a.slices;
-        const long long row = (static_cast<long long>(ahead.b) * a.Hkv + h) * a.S_cap + t0;
-        if (lane == 0) {
-            const uint32_t bytes = rows * C::kRow;
-            mbar_arrive_expect_tx(bar, 2 * bytes);
-            if (a.stream_once) {
-                bulk_copy_g2s(buf, a.kq + row * C::kRow, bytes, bar, policy);
-                bulk_copy_g2s(buf + C::kKV, a.vq + row * C::kRow, bytes, bar, policy);
-            } else {
-                bulk_copy_g2s_plain(buf, a.kq + row * C::kRow, bytes, bar);
-                bulk_copy_g2s_plain(buf + C::kKV, a.vq + row * C::kRow, bytes, bar);
-            }
-        }
-        const uint32_t sc = smem_addr(buf + 2 * C::kKV);
-#pragma unroll
-        for (int r = lane; r < C::kTile; r += 32) {
-            const bool real = r < rows;
-            const long long p = (row + (real ? r : 0)) * C::kNS;
-            cp_async_zfill<4 * C::kNS>(sc + r * 4 * C::kNS, a.ks + p, real);
-            cp_async_zfill<4 * C::kNS>(sc + C::kSc + r * 4 * C::kNS, a.vs + p, real);
-        }
-        cp_async_arrive(bar);
-        ++issued;
-        next += kI4Warps;
+    const unsigned each = static_cast<unsigned>(n) / ctas, more = static_cast<unsigned>(n) - each * ctas;
+    const int g0 = cta * each + (cta < more ? cta : more);
+    const int g1 = g0 + each + (cta < more ? 1 : 0);
+    auto cta_of = [&](unsigned tile) {
+        const unsigned edge = more * (each + 1);
+        return tile < edge ? tile / (each + 1) : more + (tile - edge) / each;
     };
-    for (int i = 0; i < C::kStages; ++i) issue();
+    const int w0 = g0 + (g1 - g0) * warp / nw, w1 = g0 + (g1 - g0) * (warp + 1) / nw;
 
-    int taken = 0;
-    bool dead = false;  // a wait ran out: the results become NaN, nothing more is waited for
-    long long mine = g0 + warp;
+    UnitWalk walk;  // of the unit being worked on
+    walk.start = 0;
+    walk.b = 0;
+    walk.u = 0;
+    walk.len = walk.nt = 0;
+    if (w0 < w1) {
+        if (a.lengths == nullptr) {
+            const unsigned each_b = per_seq * ((a.S + kGranule - 1) / kGranule);
+            walk.b = static_cast<unsigned>(w0) / each_b;
+            walk.start = walk.b * each_b;
+        } else {
+            for (int base = 0; base < a.B; base += 32) {
+                const int b = base + lane;
+                int x = base == 0 ? of_lane
+                        : b < a.B ? (i4_length(a, b) + kGranule - 1) / kGranule
+                                  : 0;
+                x *= per_seq;
+#pragma unroll
+                for (int off = 1; off < 32; off <<= 1) {
+                    const int y = __shfl_up_sync(0xffffffffu, x, off);
+                    if (lane >= off) x += y;
+                }
+                // sequences of these 32 that end at or before w0
+                const int k = __popc(__ballot_sync(0xffffffffu, walk.start + x <= w0));
+                if (k > 0) {
+                    walk.start += __shfl_sync(0xffffffffu, x, k - 1);
+                    walk.b = base + k;
+                }
+                if (k < 32) break;
+            }
+        }
+        walk.load(a);
+        walk.u = static_cast<unsigned>(w0 - walk.start) / static_cast<unsigned>(walk.nt);
+        walk.start += walk.u * walk.nt;
+    }
+    if (lane < 2) cuts[2 * warp + lane].start = w0 < w1 ? -1 : -2;
+    __syncwarp();
 
-    for (long long p0 = g0; p0 < g1;) {
-        // ---- one piece: the CTA's tiles [p0, p1) of one unit
-        walk.seek(a, p0);
-        const long long unit_end = walk.start + walk.nt;
-        const long long p1 = unit_end < g1 ? unit_end : g1;
-        const int kvh = walk.u / a.slices, slice = walk.u - kvh * a.slices;
+    // ---- the warp's stream of tiles, each of up to kM granules of one unit
+    constexpr int kChunks = C::kRow / 16;          // 16-byte chunks a row
+    constexpr int kRowsPerCopy = 32 / kChunks;     // rows one cp.async of the warp covers
+    const int copy_row = lane / kChunks;
+    // chunk i of row t stands at i ^ (t / 2 % 4), or i ^ (t / 4 % 2) for D = 64
+    const int copy_pos = (lane % kChunks) ^ (C::kSub == 4 ? (copy_row >> 1) & 3 : (copy_row >> 2) & 1);
+    const uint32_t copy_dst = smem_addr(ring) + copy_row * C::kRow + copy_pos * 16;
+    const uint32_t par_dst = smem_addr(ring) + 2 * C::kKV + lane * 4 * C::kNS;
+    UnitWalk ahead = walk;
+    int next = w0, ahead_left = 0;      // granule behind the unit's part; its rows not yet asked for
+    const uint8_t* k_src = nullptr;     // where the next tile's rows are, this lane's part
+    const uint32_t* kp_src = nullptr;
+    const long long k_to_v = a.vq - a.kq, kp_to_vp = a.vs - a.ks;
+    uint32_t fill = 0;                  // offset of the stage to fill next
+    auto issue = [&]() {
+        if (ahead_left <= 0 && next < w1) {
+            ahead.seek(a, next);
+            const int t0 = (next - ahead.start) * kGranule;
+            next = ahead.start + ahead.nt < w1 ? ahead.start + ahead.nt : w1;
+            const int rows = (next - ahead.start) * kGranule;
+            ahead_left = (rows < ahead.len ? rows : ahead.len) - t0;
+            const long long row =
+                (static_cast<long long>(ahead.b) * a.Hkv + ahead.u / a.slices) * a.S_cap + t0;
+            k_src = a.kq + row * C::kRow + lane * 16;
+            kp_src = a.ks + (row + lane) * C::kNS;
+        }
+        if (ahead_left > 0) {
+            const uint8_t* v_src = k_src + k_to_v;
+            const uint32_t* vp_src = kp_src + kp_to_vp;
+            const uint32_t dst = copy_dst + fill, pdst = par_dst + fill;
+            if (ahead_left >= C::kTile) {
+#pragma unroll
+                for (int i = 0; i < C::kKV / 512; ++i) {
+                    cp_async<16>(dst + i * 512, k_src + i * 512);
+                    cp_async<16>(dst + C::kKV + i * 512, v_src + i * 512);
+                }
+#pragma unroll
+                for (int i = 0; i < C::kTile / 32; ++i) {
+                    cp_async<4 * C::kNS>(pdst + i * 128 * C::kNS, kp_src + i * 32 * C::kNS);
+                    cp_async<4 * C::kNS>(pdst + C::kSc + i * 128 * C::kNS, vp_src + i * 32 * C::kNS);
+                }
+            } else {
+                // rows that are not the run's: zeros, addressed at the tile's first row
+#pragma unroll 1
+                for (int i = 0; i < C::kKV / 512; ++i) {
+                    const bool real = copy_row + i * kRowsPerCopy < ahead_left;
+                    const int o = real ? i * 512 : -copy_row * C::kRow;
+                    cp_async<16>(dst + i * 512, k_src + o, real);
+                    cp_async<16>(dst + C::kKV + i * 512, v_src + o, real);
+                }
+#pragma unroll
+                for (int i = 0; i < C::kTile / 32; ++i) {
+                    const bool real = lane + i * 32 < ahead_left;
+                    const int o = (real ? i * 32 : -lane) * C::kNS;
+                    cp_async<4 * C::kNS>(pdst + i * 128 * C::kNS, kp_src + o, real);
+                    cp_async<4 * C::kNS>(pdst + C::kSc + i * 128 * C::kNS, vp_src + o, real);
+                }
+            }
+            ahead_left -= C::kTile;
+            k_src += C::kKV;
+            kp_src += C::kTile * C::kNS;
+            fill += C::kStage;
+            if (fill == a.stages * C::kStage) fill = 0;
+        }
+        cp_async_commit();  // a group for every tile, real or not, so that groups can be counted
+    };
+    // ---- the query heads of a unit, as they are in memory: lane (g, c) takes 8
+    // elements of every 32 of head g; asked for ahead of the tiles
+    uint4 q_raw[NT][C::kSub];
+    auto load_q = [&](const UnitWalk& unit) {
+        const int kvh = unit.u / a.slices, slice = unit.u - kvh * a.slices;
+        const int left = a.group - slice * C::kQ;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const bool has = t * 8 + g < left;
+            const uint4* src = reinterpret_cast<const uint4*>(
+                a.q + (static_cast<long long>(unit.b) * a.Hq + kvh * a.group + slice * C::kQ +
+                       (has ? t * 8 + g : 0)) * D);
+#pragma unroll
+            for (int b = 0; b < C::kSub; ++b)
+                q_raw[t][b] = has ? src[b * 4 + c] : make_uint4(0, 0, 0, 0);
+        }
+    };
+    if (w0 < w1) load_q(walk);
+#pragma unroll 1
+    for (int i = 0; i < a.stages; ++i) issue();
+
+    const uint8_t* buf = ring;
+    // this lane's place in a tile: row g's and row 2c's chunks
+    const int k_at = g * C::kRow + (C::kSub == 4 ? (c ^ ((g >> 1) & 3)) * 16
+                                                 : (((c >> 1) ^ ((g >> 2) & 1)) * 16 + (c & 1) * 8));
+    const int v_at = 2 * c * C::kRow + (C::kSub == 4 ? ((g >> 1) ^ c) * 16
+                                                     : (((g >> 2) ^ (c >> 1)) * 16 + ((g >> 1) & 1) * 8));
+
+    for (int mine = w0; mine < w1;) {
+        // ---- one piece: the warp's granules [mine, p1) of one unit
+        const UnitWalk cur = walk;
+        const int unit_end = cur.start + cur.nt;
+        const int p1 = unit_end < w1 ? unit_end : w1;
+        const bool whole = mine == cur.start && p1 == unit_end;
+        const bool began_before = mine != cur.start;
+        const int kvh = cur.u / a.slices, slice = cur.u - kvh * a.slices;
         const int head0 = kvh * a.group + slice * C::kQ;
         const int nq = a.group - slice * C::kQ < C::kQ ? a.group - slice * C::kQ : C::kQ;
 
         // ---- q of the unit as the products' right operands
-        uint32_t qf[NT][C::kSub][2][2];
-        float qsum[NT][C::kNS][2], sc[NT][2];
+        uint32_t qf[NT][C::kSub][2][2], qz[NT];
+        float sc[NT][2];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            const bool has = t * 8 + g < nq;
             float f[C::kSub][8];
             float amax = 0.0f;
-            const uint4* src = reinterpret_cast<const uint4*>(
-                a.q + (static_cast<long long>(walk.b) * a.Hq + head0 + (has ? t * 8 + g : 0)) * D);
 #pragma unroll
             for (int b = 0; b < C::kSub; ++b) {
-                uint4 raw = make_uint4(0, 0, 0, 0);
-                if (has) raw = src[b * 4 + c];
-                if (bf16) unpack8<true>(raw, f[b]);
-                else unpack8<false>(raw, f[b]);
+                if (bf16) unpack8<true>(q_raw[t][b], f[b]);
+                else unpack8<false>(q_raw[t][b], f[b]);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(f[b][i]));
             }
@@ -336,22 +468,26 @@ __global__ void __launch_bounds__(kI4Threads, NT == 1 ? 4 : 2)
                 qf[t][b][1][0] = pack2<false>(f[b][1] * 0.0625f, f[b][5] * 0.0625f);
                 qf[t][b][1][1] = pack2<false>(f[b][3] * 0.0625f, f[b][7] * 0.0625f);
             }
-            // the scores' columns in this lane are heads 2c and 2c + 1
+            // block c's sum (below 2^18) * 2^-6 as a sum of two fp16, against its zero twice
+            float mine_sum = 0.0f;
 #pragma unroll
             for (int s = 0; s < C::kNS; ++s) {
                 sum[s] += __shfl_xor_sync(0xffffffffu, sum[s], 1);
                 sum[s] += __shfl_xor_sync(0xffffffffu, sum[s], 2);
-                sum[s] *= 5.9604644775390625e-08f;  // 2^-24, as the codes
-                qsum[t][s][0] = __shfl_sync(0xffffffffu, sum[s], 8 * c);
-                qsum[t][s][1] = __shfl_sync(0xffffffffu, sum[s], 8 * c + 4);
+                if (c == s) mine_sum = sum[s] * 0.015625f;
             }
+            const float high = __half2float(__float2half_rn(mine_sum));
+            qz[t] = pack2<false>(high, mine_sum - high);
+            // the scores' columns in this lane are heads 2c and 2c + 1
             const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23) * 16777216.0f *
                                a.score_scale;
             sc[t][0] = __shfl_sync(0xffffffffu, down, 8 * c);
             sc[t][1] = __shfl_sync(0xffffffffu, down, 8 * c + 4);
         }
 
-        float acc[NT][C::kSub][2][4], zsum[NT][C::kNS][2], M[NT][2], l[NT][2];
+        // M: largest score (base 2) that the weights are taken from; R = M + e - 11
+        float acc[NT][C::kSub][2][4], zsum[NT][C::kNS][2], M[NT][2], R[NT][2], l[NT][2];
+        float scale_top = 0.0f;  // 2^e
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
 #pragma unroll
@@ -360,40 +496,44 @@ __global__ void __launch_bounds__(kI4Threads, NT == 1 ? 4 : 2)
                 for (int i = 0; i < 8; ++i) acc[t][b][i >> 2][i & 3] = 0.0f;
 #pragma unroll
             for (int s = 0; s < C::kNS; ++s) zsum[t][s][0] = zsum[t][s][1] = 0.0f;
-            M[t][0] = M[t][1] = -INFINITY;
+            M[t][0] = M[t][1] = R[t][0] = R[t][1] = -INFINITY;
             l[t][0] = l[t][1] = 0.0f;
         }
 
-        // ---- the warp's tiles of the piece
-        for (; mine < p1; mine += kI4Warps) {
-            const int st = taken % C::kStages;
-            const uint8_t* buf = ring + st * C::kStage;
-            if (!dead && !mbar_wait_bounded(bars + st, (taken / C::kStages) & 1)) {
-                dead = true;
-                if (lane == 0) record_device_error(kErrFullWaitTimeout);
-            }
-            dead = __any_sync(0xffffffffu, dead);
-            const int left = walk.len - static_cast<int>(mine - walk.start) * C::kTile;
-            const uint32_t* kp = reinterpret_cast<const uint32_t*>(buf + 2 * C::kKV);
-            const uint32_t* vp = kp + C::kSc / 4;
+        // ---- the piece's tiles
+        const int piece_rows = (p1 - cur.start) * kGranule < cur.len ? (p1 - cur.start) * kGranule : cur.len;
+        for (int left = piece_rows - (mine - cur.start) * kGranule; left > 0; left -= C::kTile) {
+            if (a.stages == 3) cp_async_wait<2>();
+            else cp_async_wait<1>();
+            __syncwarp();
+            const uint8_t* kp = buf + 2 * C::kKV + g * 4 * C::kNS;
+            const uint8_t* vp = kp + C::kSc;
 
-            // scores of the tile, in units where 2^(x * sc) is the weight
+            // scores of the tile, in units where 2^(s * sc) is the weight
             float s[NT][C::kM][4];
 #pragma unroll
             for (int m = 0; m < C::kM; ++m) {
-                uint32_t w0[C::kSub], w1[C::kSub];
-                const uint8_t* r0 = buf + (m * 16 + g) * C::kRow + c * (C::kRow / 4);
-                if constexpr (C::kSub == 4) {
-                    *reinterpret_cast<uint4*>(w0) = *reinterpret_cast<const uint4*>(r0);
-                    *reinterpret_cast<uint4*>(w1) = *reinterpret_cast<const uint4*>(r0 + 8 * C::kRow);
-                } else {
-                    *reinterpret_cast<uint2*>(w0) = *reinterpret_cast<const uint2*>(r0);
-                    *reinterpret_cast<uint2*>(w1) = *reinterpret_cast<const uint2*>(r0 + 8 * C::kRow);
+                uint32_t w0[C::kSub], w1[C::kSub], q0[C::kNS], q1[C::kNS];
+                lds_words(w0, buf + k_at + m * 16 * C::kRow);
+                lds_words(w1, buf + k_at + (m * 16 + 8) * C::kRow);
+                lds_words(q0, kp + m * 16 * 4 * C::kNS);
+                lds_words(q1, kp + (m * 16 + 8) * 4 * C::kNS);
+                // zero terms: block c's zero twice, against the two words of its sum of q
+                uint32_t z0 = q0[0], z1 = q1[0];
+                if constexpr (C::kNS > 1) {
+                    z0 = *reinterpret_cast<const uint32_t*>(kp + (m * 16 * C::kNS + c % C::kNS) * 4);
+                    z1 = *reinterpret_cast<const uint32_t*>(kp + ((m * 16 + 8) * C::kNS + c % C::kNS) * 4);
                 }
+                z0 = __byte_perm(z0, z0, 0x3232);
+                z1 = __byte_perm(z1, z1, 0x3232);
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
+                for (int t = 0; t < NT; ++t) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) s[t][m][i] = 0.0f;
+                    mma_f16(s[t][m], z0, z1, 0u, 0u, qz[t], 0u);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[t][m][i] *= 3.814697265625e-06f;  // 2^(6 - 24)
+                }
                 float d[NT][4];
 #pragma unroll
                 for (int b = 0; b < C::kSub; ++b) {
@@ -413,17 +553,13 @@ __global__ void __launch_bounds__(kI4Threads, NT == 1 ? 4 : 2)
                     }
                     if ((b + 1) % (BS / 32) == 0) {
                         const int blk = b * 32 / BS;
-                        const uint32_t p0w = kp[(m * 16 + g) * C::kNS + blk];
-                        const uint32_t p1w = kp[(m * 16 + g + 8) * C::kNS + blk];
-                        const float2 a0 = __half22float2(*reinterpret_cast<const __half2*>(&p0w));
-                        const float2 a1 = __half22float2(*reinterpret_cast<const __half2*>(&p1w));
+                        const float a0 = __low2float(*reinterpret_cast<const __half2*>(&q0[blk]));
+                        const float a1 = __low2float(*reinterpret_cast<const __half2*>(&q1[blk]));
 #pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            s[t][m][0] = fmaf(d[t][0], a0.x, fmaf(a0.y, qsum[t][blk][0], s[t][m][0]));
-                            s[t][m][1] = fmaf(d[t][1], a0.x, fmaf(a0.y, qsum[t][blk][1], s[t][m][1]));
-                            s[t][m][2] = fmaf(d[t][2], a1.x, fmaf(a1.y, qsum[t][blk][0], s[t][m][2]));
-                            s[t][m][3] = fmaf(d[t][3], a1.x, fmaf(a1.y, qsum[t][blk][1], s[t][m][3]));
-                        }
+                        for (int t = 0; t < NT; ++t)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                s[t][m][i] = fmaf(d[t][i], i < 2 ? a0 : a1, s[t][m][i]);
                     }
                 }
             }
@@ -437,39 +573,40 @@ __global__ void __launch_bounds__(kI4Threads, NT == 1 ? 4 : 2)
                     }
             }
 
-            // ---- reference of the weights
-            float vsc[C::kM][2][C::kNS], vz[C::kM][2][C::kNS];
-            float top[NT][2];
-#pragma unroll
-            for (int t = 0; t < NT; ++t) top[t][0] = top[t][1] = -INFINITY;
+            // ---- do the references still hold?
+            __half2 big = __half2half2(__ushort_as_half(0));
 #pragma unroll
             for (int m = 0; m < C::kM; ++m)
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    float big = 0.0f;
+                    uint32_t vpar[C::kNS];
+                    lds_words(vpar, vp + (m * 16 + 8 * r) * 4 * C::kNS);
 #pragma unroll
-                    for (int k = 0; k < C::kNS; ++k) {
-                        const uint32_t pw = vp[(m * 16 + g + 8 * r) * C::kNS + k];
-                        const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&pw));
-                        vsc[m][r][k] = p.x;
-                        vz[m][r][k] = p.y;
-                        big = fmaxf(big, p.x);
-                    }
-                    // exponent of the power of two above the scale, at least
-                    // -24 (fp16's smallest step; blocks of one value have scale 0)
-                    const float et = fmaxf(
-                        __uint_as_float(0x4b000000u | (__float_as_uint(big) >> 23)) - 8388734.0f,
-                        -24.0f);
-#pragma unroll
-                    for (int t = 0; t < NT; ++t)
-#pragma unroll
-                        for (int j = 0; j < 2; ++j)
-                            top[t][j] = fmaxf(top[t][j], fmaf(s[t][m][2 * r + j], sc[t][j], et));
+                    for (int k = 0; k < C::kNS; ++k)
+                        big = __hmax2(big, *reinterpret_cast<const __half2*>(&vpar[k]));
                 }
-            bool over = false;
+            bool over = __low2float(big) > scale_top;
+            float top[NT][2];
 #pragma unroll
-            for (int t = 0; t < NT; ++t) over |= top[t][0] > M[t][0] + 4.0f || top[t][1] > M[t][1] + 4.0f;
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    top[t][j] = fmaxf(s[t][0][j], s[t][0][j + 2]);
+#pragma unroll
+                    for (int m = 1; m < C::kM; ++m)
+                        top[t][j] = fmaxf(top[t][j], fmaxf(s[t][m][j], s[t][m][j + 2]));
+                    top[t][j] *= sc[t][j];
+                    over |= top[t][j] > M[t][j] + 4.0f;
+                }
             if (__any_sync(0xffffffffu, over)) {
+                float bigf = fmaxf(__low2float(big), 5.9604644775390625e-08f);
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1)
+                    bigf = fmaxf(bigf, __shfl_xor_sync(0xffffffffu, bigf, off));
+                // the power of two above, and its exponent
+                scale_top = fmaxf(scale_top,
+                                  __uint_as_float((__float_as_uint(bigf) + 0x00800000u) & 0x7f800000u));
+                const float e = static_cast<float>(static_cast<int>(__float_as_uint(scale_top) >> 23) - 127);
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -478,9 +615,10 @@ __global__ void __launch_bounds__(kI4Threads, NT == 1 ? 4 : 2)
 #pragma unroll
                         for (int off = 4; off < 32; off <<= 1)
                             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
-                        x = fmaxf(x, M[t][j]);
-                        const float f = x == M[t][j] ? 1.0f : fast_exp2(M[t][j] - x);
-                        M[t][j] = x;
+                        M[t][j] = fmaxf(x, M[t][j]);
+                        const float r = M[t][j] + e - 11.0f;
+                        const float f = r == R[t][j] ? 1.0f : fast_exp2(R[t][j] - r);
+                        R[t][j] = r;
                         l[t][j] *= f;
 #pragma unroll
                         for (int k = 0; k < C::kNS; ++k) zsum[t][k][j] *= f;
@@ -497,58 +635,75 @@ __global__ void __launch_bounds__(kI4Threads, NT == 1 ? 4 : 2)
             // ---- weights and the second product
 #pragma unroll
             for (int m = 0; m < C::kM; ++m) {
-                uint32_t bw[NT][C::kNS][2];
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    float p[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        p[i] = fast_exp2(fmaf(s[t][m][i], sc[t][i & 1], 11.0f - M[t][i & 1]));
-                    l[t][0] += p[0] + p[2];
-                    l[t][1] += p[1] + p[3];
-#pragma unroll
-                    for (int k = 0; k < C::kNS; ++k) {
-                        bw[t][k][0] = movmatrix(pack2<false>(p[0] * vsc[m][0][k], p[1] * vsc[m][0][k]));
-                        bw[t][k][1] = movmatrix(pack2<false>(p[2] * vsc[m][1][k], p[3] * vsc[m][1][k]));
-                        zsum[t][k][0] = fmaf(p[0], vz[m][0][k], fmaf(p[2], vz[m][1][k], zsum[t][k][0]));
-                        zsum[t][k][1] = fmaf(p[1], vz[m][0][k], fmaf(p[3], vz[m][1][k], zsum[t][k][1]));
-                    }
-                }
-                // tokens 2c, 2c + 1, 2c + 8, 2c + 9 of the piece; this lane's 16
-                // bits of each 32-element group
-                const uint8_t* v0 = buf + C::kKV + (m * 16 + 2 * c) * C::kRow + (g >> 1) * (C::kRow / 4);
+                uint32_t q0[C::kNS], q1[C::kNS];  // parameters of rows g, g + 8
+                lds_words(q0, vp + m * 16 * 4 * C::kNS);
+                lds_words(q1, vp + (m * 16 + 8) * 4 * C::kNS);
+                // tokens 2c, 2c + 1, 2c + 8, 2c + 9 of the 16; this lane's 16 bits
+                // of each 32-element group
                 uint32_t x[4][C::kSub];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint8_t* src = v0 + ((i & 1) + (i >> 1) * 8) * C::kRow;
-                    if constexpr (C::kSub == 4)
-                        *reinterpret_cast<uint4*>(x[i]) = *reinterpret_cast<const uint4*>(src);
-                    else
-                        *reinterpret_cast<uint2*>(x[i]) = *reinterpret_cast<const uint2*>(src);
-                }
+                for (int i = 0; i < 4; ++i)
+                    lds_words(x[i], buf + C::kKV + v_at + (m * 16 + (i & 1) + (i >> 1) * 8) * C::kRow);
                 const uint32_t sel = (g & 1) ? 0x7632u : 0x5410u;
+                float p[NT][4];
 #pragma unroll
-                for (int b = 0; b < C::kSub; ++b) {
-                    const int k = b * 32 / BS;
-                    const uint32_t lo = __byte_perm(x[0][b], x[1][b], sel);
-                    const uint32_t hi = __byte_perm(x[2][b], x[3][b], sel);
-                    const uint32_t lo8 = lo >> 8, hi8 = hi >> 8;
+                for (int t = 0; t < NT; ++t) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        p[t][i] = fast_exp2(fmaf(s[t][m][i], sc[t][i & 1], -R[t][i & 1]));
+                    l[t][0] += p[t][0] + p[t][2];
+                    l[t][1] += p[t][1] + p[t][3];
+                }
+#pragma unroll
+                for (int k = 0; k < C::kNS; ++k) {
+                    float2 va = __half22float2(*reinterpret_cast<const __half2*>(&q0[k]));
+                    float2 vb = __half22float2(*reinterpret_cast<const __half2*>(&q1[k]));
+                    va.y = fmaf(va.x, 8.0f, va.y);  // zero + 8 scale
+                    vb.y = fmaf(vb.x, 8.0f, vb.y);
+                    uint32_t bw[NT][2];
 #pragma unroll
                     for (int t = 0; t < NT; ++t) {
-                        mma_f16(acc[t][b][0], lo & 0x000f000fu, lo8 & 0x000f000fu, hi & 0x000f000fu,
-                                hi8 & 0x000f000fu, bw[t][k][0], bw[t][k][1]);
-                        mma_f16(acc[t][b][1], lo & 0x00f000f0u, lo8 & 0x00f000f0u, hi & 0x00f000f0u,
-                                hi8 & 0x00f000f0u, bw[t][k][0], bw[t][k][1]);
+                        bw[t][0] = movmatrix(pack2<false>(p[t][0] * va.x, p[t][1] * va.x));
+                        bw[t][1] = movmatrix(pack2<false>(p[t][2] * vb.x, p[t][3] * vb.x));
+                        zsum[t][k][0] = fmaf(p[t][0], va.y, fmaf(p[t][2], vb.y, zsum[t][k][0]));
+                        zsum[t][k][1] = fmaf(p[t][1], va.y, fmaf(p[t][3], vb.y, zsum[t][k][1]));
+                    }
+#pragma unroll
+                    for (int b = k * BS / 32; b < (k + 1) * BS / 32; ++b) {
+                        const uint32_t lo = __byte_perm(x[0][b], x[1][b], sel);
+                        const uint32_t hi = __byte_perm(x[2][b], x[3][b], sel);
+                        const uint32_t lo8 = lo >> 8, hi8 = hi >> 8;
+                        const uint32_t a0 = minus8<24>(lo), a1 = minus8<24>(lo8);
+                        const uint32_t a2 = minus8<24>(hi), a3 = minus8<24>(hi8);
+                        const uint32_t c0 = minus8<20>(lo), c1 = minus8<20>(lo8);
+                        const uint32_t c2 = minus8<20>(hi), c3 = minus8<20>(hi8);
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) {
+                            mma_f16(acc[t][b][0], a0, a1, a2, a3, bw[t][0], bw[t][1]);
+                            mma_f16(acc[t][b][1], c0, c1, c2, c3, bw[t][0], bw[t][1]);
+                        }
                     }
                 }
             }
-            ++taken;
+            buf += C::kStage;
+            if (buf == ring + a.stages * C::kStage) buf = ring;
             __syncwarp();  // every lane is done with the stage: refill it
-            if (!dead) issue();
+            issue();
         }
 
-        // ---- the warp's state to shared memory: acc[D], l, M per query head
-        const int rows = a.rec_rows;
+        mine = p1;
+        if (mine < w1) {
+            walk.seek(a, mine);
+            load_q(walk);
+        }
+
+        // ---- the piece's state: to O, or to shared memory as acc[D], l, R per head
+        const bool behind = !whole && !began_before;  // goes on behind the run: the ring is used up
+        float* slot = behind ? reinterpret_cast<float*>(ring) : merge + warp * state_floats;
+        if (behind) __syncwarp();
+        if (!whole && lane == 0)
+            cuts[2 * warp + (behind ? 1 : 0)] =
+                CutUnit{cur.start, unit_end, cur.b * a.Hq + head0, nq};
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -565,119 +720,203 @@ __global__ void __launch_bounds__(kI4Threads, NT == 1 ? 4 : 2)
                         zs[k] += __shfl_xor_sync(0xffffffffu, zs[k], off);
                 }
                 const int r = t * 8 + 2 * c + j;
-                if (r < nq) {
-                    float* dst = merge + (warp * rows + r) * C::kRecStride;
+                if (r >= nq) continue;
+                const float inv = whole ? 1.0f / ls : 1.0f;
 #pragma unroll
-                    for (int b = 0; b < C::kSub; ++b) {
-                        const float z = zs[b * 32 / BS];
-                        float4 v;  // elements 32 b + 4 g + {0, 1, 2, 3}
-                        v.x = fmaf(acc[t][b][0][j], 16777216.0f, z);
-                        v.y = fmaf(acc[t][b][1][j], 1048576.0f, z);
-                        v.z = fmaf(acc[t][b][0][j + 2], 16777216.0f, z);
-                        v.w = fmaf(acc[t][b][1][j + 2], 1048576.0f, z);
-                        *reinterpret_cast<float4*>(dst + 32 * b + 4 * g) = v;
-                    }
-                    if (g == 0) {
-                        dst[D] = dead ? NAN : ls;
-                        dst[D + 1] = M[t][j];
-                    }
+                for (int b = 0; b < C::kSub; ++b) {
+                    const float z = zs[b * 32 / BS];
+                    float4 v;  // elements 32 b + 4 g + {0, 1, 2, 3}
+                    v.x = fmaf(acc[t][b][0][j], 16777216.0f, z) * inv;
+                    v.y = fmaf(acc[t][b][1][j], 1048576.0f, z) * inv;
+                    v.z = fmaf(acc[t][b][0][j + 2], 16777216.0f, z) * inv;
+                    v.w = fmaf(acc[t][b][1][j + 2], 1048576.0f, z) * inv;
+                    if (whole)
+                        store_out(a.o + (static_cast<long long>(cur.b) * a.Hq + head0 + r) * D + 32 * b + 4 * g,
+                                  v, bf16);
+                    else
+                        *reinterpret_cast<float4*>(slot + r * C::kRecStride + 32 * b + 4 * g) = v;
                 }
+                if (!whole && g == 0)
+                    *reinterpret_cast<float2*>(slot + r * C::kRecStride + D) = make_float2(ls, R[t][j]);
             }
-        __syncthreads();
+    }
+    __syncthreads();
 
-        // ---- the CTA's state: thread (row, 4 elements)
-        constexpr int kLanes = D / 4;
-        const bool whole = walk.start >= g0 && unit_end <= g1;
-        const bool starts_here = walk.start >= g0;
-        for (int r = threadIdx.x / kLanes; r < nq; r += kI4Threads / kLanes) {
-            const int i = threadIdx.x % kLanes;
-            const float* src = merge + r * C::kRecStride;
-            float m = -INFINITY;
+    // ---- join the states of the units that the CTA's warps cut.  A unit's first
+    // state here is warp 0's first (it began before the CTA) or some warp's second;
+    // the first states of the warps behind it follow while they are of the unit.
+    // A warp joins a row; lane w knows warp w's descriptors.
+    constexpr int kLanes = D / 4;  // lanes a row takes, 4 elements each
+    constexpr int kSide = 32 / kLanes;
+    const int i = lane % kLanes, side = lane / kLanes;
+    const CutUnit before = cuts[0];
+    const int first_of = lane < nw ? cuts[2 * lane].start : -1;
+    const unsigned begins = __ballot_sync(0xffffffffu, lane < nw && cuts[2 * (lane % nw) + 1].start >= 0);
+    const unsigned idle = __ballot_sync(0xffffffffu, first_of == -2);
+    int turn = warp;  // rows go round the warps
+    unsigned todo = begins;
+    for (bool lead = before.start >= 0; lead || todo != 0; lead = false) {
+        const int w = lead ? 0 : __ffs(todo) - 1;
+        if (!lead) todo &= todo - 1;
+        const CutUnit unit = lead ? before : cuts[2 * w + 1];
+        const float* head = lead ? merge : reinterpret_cast<const float*>(smem + w * ring_bytes);
+        const unsigned of_unit = __ballot_sync(0xffffffffu, first_of == unit.start);
+        const int from = w + 1, count = __ffs(~((of_unit | idle) >> from)) - 1;
+        const unsigned set = of_unit & (((1u << count) - 1u) << from);
+        int r = turn;
+        for (; r < unit.nq; r += nw) {
+            // lane w: the state of warp w; lane 31: the first
+            const bool have = lane == 31 || (set >> lane & 1u);
+            float2 lr = make_float2(0.0f, -INFINITY);
+            if (have)
+                lr = *reinterpret_cast<const float2*>((lane == 31 ? head : merge + lane * state_floats) +
+                                                      r * C::kRecStride + D);
+            float m = lr.y;
 #pragma unroll
-            for (int w = 0; w < kI4Warps; ++w) m = fmaxf(m, src[w * rows * C::kRecStride + D + 1]);
-            float4 v = make_float4(0, 0, 0, 0);
-            float ls = 0.0f;
+            for (int off = 16; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+            const float f = lr.y == -INFINITY && lr.x == 0.0f ? 0.0f : fast_exp2(lr.y - m);
+            float ls = lr.x * f;
 #pragma unroll
-            for (int w = 0; w < kI4Warps; ++w) {
-                const float* p = src + w * rows * C::kRecStride;
-                if (p[D + 1] == -INFINITY && p[D] == 0.0f) continue;  // a warp without tiles
-                const float f = fast_exp2(p[D + 1] - m);
-                const float4 x = *reinterpret_cast<const float4*>(p + 4 * i);
-                v.x = fmaf(x.x, f, v.x);
-                v.y = fmaf(x.y, f, v.y);
-                v.z = fmaf(x.z, f, v.z);
-                v.w = fmaf(x.w, f, v.w);
-                ls = fmaf(p[D], f, ls);
+            for (int off = 16; off; off >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, off);
+            float4 v = *reinterpret_cast<const float4*>(head + r * C::kRecStride + 4 * i);
+            float fw = __shfl_sync(0xffffffffu, f, 31);
+            v.x *= fw, v.y *= fw, v.z *= fw, v.w *= fw;
+#pragma unroll 4
+            for (int k = from; k < from + count; ++k) {
+                float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (set >> k & 1u)
+                    x = *reinterpret_cast<const float4*>(merge + k * state_floats + r * C::kRecStride + 4 * i);
+                fw = __shfl_sync(0xffffffffu, f, k);
+                v.x = fmaf(x.x, fw, v.x);
+                v.y = fmaf(x.y, fw, v.y);
+                v.z = fmaf(x.z, fw, v.z);
+                v.w = fmaf(x.w, fw, v.w);
             }
-            if (whole) {
+            if (side != 0) continue;
+            if (unit.start >= g0 && unit.end <= g1) {
                 const float inv = 1.0f / ls;
-                uint2 out;
-                out.x = bf16 ? pack2<true>(v.x * inv, v.y * inv) : pack2<false>(v.x * inv, v.y * inv);
-                out.y = bf16 ? pack2<true>(v.z * inv, v.w * inv) : pack2<false>(v.z * inv, v.w * inv);
-                reinterpret_cast<uint2*>(a.o + (static_cast<long long>(walk.b) * a.Hq + head0 + r) * D)[i] = out;
+                store_out(a.o + static_cast<long long>(unit.row + r) * D + 4 * i,
+                          make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv), bf16);
             } else {
-                float* rec = a.recs + ((cta * 2 + (starts_here ? 1 : 0)) * rows + r) * C::kRecStride;
+                float* rec = a.recs + static_cast<long long>(cta * 2 + (unit.start >= g0 ? 1 : 0)) * state_floats +
+                             r * C::kRecStride;
                 __stcg(reinterpret_cast<float4*>(rec) + i, v);
                 if (i == 0) __stcg(reinterpret_cast<float2*>(rec + D), make_float2(ls, m));
             }
         }
+        turn = r - unit.nq;  // the rows of the next unit go on where these ended
+    }
 
-        if (!whole) {
-            // ---- the last CTA to arrive merges the unit's records
-            const long long first = cta_of(walk.start), last = cta_of(unit_end - 1);
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                __threadfence();
-                const unsigned int before = atomicAdd(a.counters + first, 1u);
-                __threadfence();
-                const bool done = before == static_cast<unsigned int>(last - first);
-                if (done) a.counters[first] = 0u;
-                *flag = done;
+    // ---- units cut across CTAs: the one that began before (0), the one that goes
+    // on behind (1); the last CTA to arrive at a unit's counter merges its records
+    CutUnit behind;
+    behind.start = -1;
+    if (begins != 0) behind = cuts[2 * (31 - __clz(begins)) + 1];
+    if (behind.start >= 0 && behind.end <= g1) behind.start = -1;
+    if (before.start < 0 && behind.start < 0) return;
+    // their first and last CTAs
+    const unsigned before_first = before.start >= 0 ? cta_of(before.start) : 0;
+    const unsigned before_last = before.end <= g1 ? cta : cta_of(before.end - 1);
+    const unsigned behind_last = behind.start >= 0 ? cta_of(behind.end - 1) : 0;
+    __syncthreads();
+    if (threadIdx.x < 2) {
+        const bool mine = (threadIdx.x == 0 ? before.start : behind.start) >= 0;
+        const unsigned first = threadIdx.x == 0 ? before_first : cta;
+        const unsigned last = threadIdx.x == 0 ? before_last : behind_last;
+        unsigned done = 0;
+        if (mine) {
+            done = arrive_acq_rel(a.counters + first) == last - first;
+            if (done) a.counters[first] = 0u;
+        }
+        flags[threadIdx.x] = done;
+    }
+    __syncthreads();
+    const bool both = flags[0] && flags[1];
+    if (!flags[0] && !flags[1]) return;
+    // all warps merge the one unit, or half of them each of the two.  A warp takes
+    // a row, or, with fewer rows than warps, a run of its pieces; the loads of 8
+    // pieces (16 for D = 64) go out together
+    const int team = both ? nw >> 1 : nw;
+    const int which = both ? (warp >= team ? 1 : 0) : (flags[0] ? 0 : 1);
+    const int member = both && which ? warp - team : warp;
+    const CutUnit unit = which == 0 ? before : behind;
+    int log_split = 0;
+    while ((unit.nq << (log_split + 1)) <= team) ++log_split;
+    const unsigned unit_first = which == 0 ? before_first : cta;
+    const int np = static_cast<int>((which == 0 ? before_last : behind_last) - unit_first) + 1;
+    const int rec_cta = 2 * state_floats;
+    float* parts = merge + (which && both ? (team > rows ? team : rows) : 0) * C::kRecStride;
+    float* rec0 = a.recs + static_cast<long long>(unit_first) * rec_cta;
+    // the first CTA's piece is its second record, all others' the first
+    auto at = [&](int p) { return rec0 + static_cast<long long>(p) * rec_cta + (p == 0 ? state_floats : 0); };
+    for (int item = member; item < unit.nq << log_split; item += team) {
+        const int r = item >> log_split, part = item - (r << log_split);
+        const int pa = np * part >> log_split, pb = np * (part + 1) >> log_split;
+        constexpr int kDeep = 8;
+        float m = -INFINITY, ls = 0.0f;
+        float4 v = make_float4(0, 0, 0, 0);
+        for (int pw = pa; pw < pb; pw += kDeep * kSide) {
+            float4 x[kDeep];
+            float2 lr = make_float2(0.0f, -INFINITY);  // of piece pw + lane
+            if (lane < kDeep * kSide && pw + lane < pb)
+                lr = __ldcg(reinterpret_cast<const float2*>(at(pw + lane) + r * C::kRecStride + D));
+#pragma unroll
+            for (int k = 0; k < kDeep; ++k) {
+                const int p = pw + k * kSide + side;
+                x[k] = make_float4(0, 0, 0, 0);
+                if (p < pb) x[k] = __ldcg(reinterpret_cast<const float4*>(at(p) + r * C::kRecStride) + i);
             }
-            __syncthreads();
-            if (*flag) {
-                const long long rec_cta = 2ll * rows * C::kRecStride;
-                for (int r = threadIdx.x / kLanes; r < nq; r += kI4Threads / kLanes) {
-                    const int i = threadIdx.x % kLanes;
-                    // the first CTA's piece is its second record, all others' the first
-                    float* rec = a.recs + (first * 2 * rows + r) * C::kRecStride;
-                    auto at = [&](long long p) {
-                        return rec + p * rec_cta + (p == 0 ? rows * C::kRecStride : 0);
-                    };
-                    const int np = static_cast<int>(last - first) + 1;
-                    float m = -INFINITY;
-#pragma unroll 4
-                    for (int p = 0; p < np; ++p) m = fmaxf(m, __ldcg(at(p) + D + 1));
-                    float4 v = make_float4(0, 0, 0, 0);
-                    float ls = 0.0f;
-#pragma unroll 4
-                    for (int p = 0; p < np; ++p) {
-                        const float2 lm = __ldcg(reinterpret_cast<const float2*>(at(p) + D));
-                        const float4 x = __ldcg(reinterpret_cast<const float4*>(at(p)) + i);
-                        const float f = fast_exp2(lm.y - m);
-                        v.x = fmaf(x.x, f, v.x);
-                        v.y = fmaf(x.y, f, v.y);
-                        v.z = fmaf(x.z, f, v.z);
-                        v.w = fmaf(x.w, f, v.w);
-                        ls = fmaf(lm.x, f, ls);
-                    }
-                    const float inv = 1.0f / ls;
-                    uint2 out;
-                    out.x = bf16 ? pack2<true>(v.x * inv, v.y * inv) : pack2<false>(v.x * inv, v.y * inv);
-                    out.y = bf16 ? pack2<true>(v.z * inv, v.w * inv) : pack2<false>(v.z * inv, v.w * inv);
-                    reinterpret_cast<uint2*>(a.o + (static_cast<long long>(walk.b) * a.Hq + head0 + r) * D)[i] = out;
-                }
-                __syncthreads();  // all reads done: the records are zero again
-                for (long long p = first; p <= last; ++p) {
-                    float4* rec = reinterpret_cast<float4*>(
-                        a.recs + (p * 2 + (p == first ? 1 : 0)) * rows * C::kRecStride);
-                    for (int i = threadIdx.x; i < nq * C::kRecStride / 4; i += kI4Threads)
-                        __stcg(rec + i, make_float4(0, 0, 0, 0));
-                }
+            float top = lr.y;
+#pragma unroll
+            for (int off = 1; off < kDeep * kSide; off <<= 1)
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+            top = fmaxf(m, __shfl_sync(0xffffffffu, top, 0));
+            const float old = m == top ? 1.0f : fast_exp2(m - top);
+            m = top;
+            const float f = lr.y == -INFINITY && lr.x == 0.0f ? 0.0f : fast_exp2(lr.y - m);
+            ls = fmaf(ls, old, lr.x * f);
+            v.x *= old, v.y *= old, v.z *= old, v.w *= old;
+#pragma unroll
+            for (int k = 0; k < kDeep; ++k) {
+                const float fk = __shfl_sync(0xffffffffu, f, k * kSide + side);
+                v.x = fmaf(x[k].x, fk, v.x);
+                v.y = fmaf(x[k].y, fk, v.y);
+                v.z = fmaf(x[k].z, fk, v.z);
+                v.w = fmaf(x[k].w, fk, v.w);
             }
         }
-        __syncthreads();  // the merge area and the flag are free again
-        p0 = p1;
+#pragma unroll
+        for (int off = 16; off; off >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, off);
+        if constexpr (kSide == 2) {
+            v.x += __shfl_xor_sync(0xffffffffu, v.x, 16);
+            v.y += __shfl_xor_sync(0xffffffffu, v.y, 16);
+            v.z += __shfl_xor_sync(0xffffffffu, v.z, 16);
+            v.w += __shfl_xor_sync(0xffffffffu, v.w, 16);
+        }
+        if (side == 0) {
+            float* dst = parts + item * C::kRecStride;
+            *reinterpret_cast<float4*>(dst + 4 * i) = v;
+            if (i == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(ls, m);
+        }
+    }
+    __syncthreads();  // all records are read
+    for (int r = member * kSide + side; r < unit.nq; r += team * kSide) {
+        const float* src = parts + (r << log_split) * C::kRecStride;
+        float4 v = *reinterpret_cast<const float4*>(src + 4 * i);
+        float2 lr = *reinterpret_cast<const float2*>(src + D);
+        for (int p = 1; p < 1 << log_split; ++p) {
+            src += C::kRecStride;
+            join(v, lr, *reinterpret_cast<const float4*>(src + 4 * i), *reinterpret_cast<const float2*>(src + D));
+        }
+        const float inv = 1.0f / lr.x;
+        store_out(a.o + static_cast<long long>(unit.row + r) * D + 4 * i,
+                  make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv), bf16);
+    }
+    // the records are zero again: nq * kRecStride floats of every piece
+    for (int p = member; p < np; p += team) {
+        float4* rec = reinterpret_cast<float4*>(at(p));
+        for (int k = lane; k < unit.nq * C::kRecStride / 4; k += 32)
+            __stcg(rec + k, make_float4(0, 0, 0, 0));
     }
 }
 

@@ -303,9 +303,12 @@ __global__ void __launch_bounds__(kInt4Threads)
 // and its reciprocal root is the fp64 one rounded to fp32; the products and
 // sums after it are rounded one by one (no contraction).
 //
-// One group of D / 8 lanes takes one token and up to `heads_per_group` heads
-// of one kind, so that the table's 64 bytes a lane (against 16 of data) are
-// read once for those heads.
+// A row is D / 16 lanes; a lane holds two runs of 8 elements such that the
+// halves of a pair meet in one lane (elements 8 l .. and rot / 2 + 8 l ..), so
+// the rotation needs no other lane, and 8 elements are one word of the 4-bit
+// format.  A lane group takes one token and up to heads_per_group heads of one
+// kind, so that the table's 64 bytes a lane (against 32 of data) are read once
+// for those heads.
 struct RopeArgs {
     const uint16_t *q, *k, *v;     // element (b, h, t, 0) at b * sb + h * sh + t * st
     long long q_sb, q_sh, q_st, k_sb, k_sh, k_st, v_sb, v_sh, v_st;
@@ -325,16 +328,65 @@ struct RopeArgs {
     FastDiv groups, divT;          // lane groups a token needs in all
 };
 
-constexpr int kRopeUnroll = 4;
+// 1 / sqrt(x) rounded to fp32 as if from its exact value: one Newton step in
+// fp64 from the fp32 approximation (relative error 2^-22, then 2^-43).
+__device__ __forceinline__ float rsqrt_rounded(double x) {
+    if (!(x > 1e-36 && x < 1e36)) return static_cast<float>(rsqrt(x));
+    const double y = rsqrtf(static_cast<float>(x));
+    return static_cast<float>(fma(0.5 * y, fma(-x * y, y, 1.0), y));
+}
+
+// Minimum and maximum of lane runs over blocks of BS elements, 8 a lane:
+// aligned groups of BS / 8 lanes when `a` and `b` are different blocks, or, for
+// BS = D, both runs of every lane of the row.
+template <int D, int BS>
+__device__ __forceinline__ void store_int4_runs(const float (&a)[8], const float (&b)[8], int l,
+                                                long long row, bool valid,
+                                                uint32_t* __restrict__ codes,
+                                                uint32_t* __restrict__ params) {
+    constexpr int kLanes = D / 16;  // lanes a row has; run a is element 8 l, run b D / 2 + 8 l
+    float lo[2] = {a[0], b[0]}, hi[2] = {a[0], b[0]};
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+        lo[0] = min_nan(lo[0], a[i]);
+        hi[0] = max_nan(hi[0], a[i]);
+        lo[1] = min_nan(lo[1], b[i]);
+        hi[1] = max_nan(hi[1], b[i]);
+    }
+    if constexpr (BS == D) {
+        lo[0] = lo[1] = min_nan(lo[0], lo[1]);
+        hi[0] = hi[1] = max_nan(hi[0], hi[1]);
+    }
+    constexpr int kGroup = BS == D ? kLanes : BS / 8;
+#pragma unroll
+    for (int h = 0; h < (BS == D ? 1 : 2); ++h)
+#pragma unroll
+        for (int off = 1; off < kGroup; off <<= 1) {
+            lo[h] = min_nan(lo[h], __shfl_xor_sync(0xffffffffu, lo[h], off));
+            hi[h] = max_nan(hi[h], __shfl_xor_sync(0xffffffffu, hi[h], off));
+        }
+    if constexpr (BS == D) lo[1] = lo[0], hi[1] = hi[0];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        uint32_t p;
+        const uint32_t w = int4_codes(h == 0 ? a : b, lo[h], hi[h], p);
+        if (!valid) continue;
+        const int run = l + h * kLanes;
+        codes[row * (D / 8) + word_of_lane<D>(run)] = w;
+        if (run % (BS / 8) == 0) params[row * (D / BS) + run / (BS / 8)] = p;
+    }
+}
+
+constexpr int kRopeUnroll = 2;  // heads whose rows a lane group has in flight
 
 template <int D, int BS, bool BF16, bool APPEND, bool INTERLEAVED>
-__global__ void __launch_bounds__(kInt4Threads) qk_norm_rope_kernel(RopeArgs a) {
+__global__ void __launch_bounds__(kInt4Threads, 2) qk_norm_rope_kernel(const RopeArgs a) {
     griddep_wait();
     griddep_launch_dependents();
-    constexpr int kLPR = D / 8;
+    constexpr int kLanes = D / 16;
     const int lane = threadIdx.x & 31;
-    const int l = lane % kLPR;
-    const uint32_t unit = (blockIdx.x * kInt4Threads + threadIdx.x) / kLPR;
+    const int l = lane % kLanes;
+    const uint32_t unit = (blockIdx.x * kInt4Threads + threadIdx.x) / kLanes;
     uint32_t tok = a.groups.div(unit);
     int grp = static_cast<int>(unit - tok * a.groups.d);
     const bool live = tok < a.tokens;
@@ -356,19 +408,24 @@ __global__ void __launch_bounds__(kInt4Threads) qk_norm_rope_kernel(RopeArgs a) 
                                     : a.v + b * a.v_sb + t * a.v_st;
     const long long sh = kind == 0 ? a.q_sh : kind == 1 ? a.k_sh : a.v_sh;
 
-    // cos and sin of the lane's pairs; its partner lane holds the pairs' other halves
-    const int half_lanes = a.rot / 16;
-    const bool rotates = l < 2 * half_lanes && kind != 2;
-    const bool second = l >= half_lanes;
-    const int partner = INTERLEAVED || !rotates ? lane : second ? lane - half_lanes
-                                                                : lane + half_lanes;
-    constexpr int kPairs = INTERLEAVED ? 4 : 8;
-    float2 cs[kPairs];
-    if (rotates) {
-        const int j0 = INTERLEAVED ? l * 4 : (second ? l - half_lanes : l) * 8;
+    // runs (in units of 8 elements): the pairs' halves of the rotated part, and
+    // the halves of what is behind it
+    const int rot_lanes = a.rot / 16;
+    const bool rotates = l < rot_lanes && kind != 2;
+    const bool natural = INTERLEAVED || a.rot == D || kind == 2;  // runs l and l + kLanes
+    const int run0 = natural || l < rot_lanes ? l : rot_lanes + l;
+    const int run1 = natural ? l + kLanes : l < rot_lanes ? rot_lanes + l : kLanes + l;
+    float2 cs[8];
+    bool turns[2] = {rotates, rotates};  // interleaved: whether run 0 and run 1 rotate
+    if (INTERLEAVED) {
+        turns[0] = kind != 2 && run0 < 2 * rot_lanes;
+        turns[1] = kind != 2 && run1 < 2 * rot_lanes;
+    }
 #pragma unroll
-        for (int i = 0; i < kPairs; ++i) {
-            const int j = j0 + i;
+    for (int i = 0; i < 8; ++i) {
+        const int j = INTERLEAVED ? (i < 4 ? run0 : run1) * 4 + (i & 3) : l * 8 + i;
+        cs[i] = make_float2(1.0f, 0.0f);
+        if (turns[INTERLEAVED ? i >> 2 : 0]) {
             const int axis = a.axes == 1 ? 0 : (j >= a.s1) + (j >= a.s2) + (j >= a.s3);
             const int p = a.pos[static_cast<long long>(axis) * a.tokens + tok];
             // a position outside the table leaves NaN in the row
@@ -378,73 +435,69 @@ __global__ void __launch_bounds__(kInt4Threads) qk_norm_rope_kernel(RopeArgs a) 
         }
     }
     const uint16_t* wsrc = kind == 0 ? a.q_w : kind == 1 ? a.k_w : nullptr;
-    uint4 w_own = make_uint4(0, 0, 0, 0), w_other = w_own;
+    float w0[8], w1[8];
     if (wsrc) {
-        w_own = reinterpret_cast<const uint4*>(wsrc)[l];
-        if (!INTERLEAVED) w_other = reinterpret_cast<const uint4*>(wsrc)[l + partner - lane];
+        unpack8<BF16>(reinterpret_cast<const uint4*>(wsrc)[run0], w0);
+        unpack8<BF16>(reinterpret_cast<const uint4*>(wsrc)[run1], w1);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w0[i] = w1[i] = 1.0f;
     }
 
+    const bool norms = __any_sync(0xffffffffu, kind != 2);   // some row of the warp is q's or k's
+    const bool caches = __any_sync(0xffffffffu, kind != 0);  // some row goes to a cache, if any does
     for (int hb = h0; __any_sync(0xffffffffu, hb < h1); hb += kRopeUnroll) {
-        uint4 raw[kRopeUnroll];
+        uint4 raw[kRopeUnroll][2];
 #pragma unroll
         for (int u = 0; u < kRopeUnroll; ++u) {
-            raw[u] = make_uint4(0, 0, 0, 0);
-            if (hb + u < h1) raw[u] = reinterpret_cast<const uint4*>(x + (hb + u) * sh)[l];
+            raw[u][0] = raw[u][1] = make_uint4(0, 0, 0, 0);
+            if (hb + u < h1) {
+                const uint4* src = reinterpret_cast<const uint4*>(x + (hb + u) * sh);
+                raw[u][0] = src[run0];
+                raw[u][1] = src[run1];
+            }
         }
 #pragma unroll
         for (int u = 0; u < kRopeUnroll; ++u) {
             const int h = hb + u;
             if (!__any_sync(0xffffffffu, h < h1)) break;
-            float f[8];
-            unpack8<BF16>(raw[u], f);
-            double ss = 0.0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const double v = f[i];
-                ss = fma(v, v, ss);
-            }
-#pragma unroll
-            for (int off = 1; off < kLPR; off <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-            const float inv = static_cast<float>(rsqrt(ss * (1.0 / D) + a.eps));
-            float g[8];
-            if constexpr (!INTERLEAVED) {
-                uint4 other;
-                other.x = __shfl_sync(0xffffffffu, raw[u].x, partner);
-                other.y = __shfl_sync(0xffffffffu, raw[u].y, partner);
-                other.z = __shfl_sync(0xffffffffu, raw[u].z, partner);
-                other.w = __shfl_sync(0xffffffffu, raw[u].w, partner);
-                unpack8<BF16>(other, g);
-            }
-            if (kind != 2) {
-                float wf[8];
-                unpack8<BF16>(w_own, wf);
+            float f0[8], f1[8];
+            unpack8<BF16>(raw[u][0], f0);
+            unpack8<BF16>(raw[u][1], f1);
+            if (norms) {
+                double ss = 0.0, st = 0.0;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    f[i] = __fmul_rn(f[i], inv);
-                    if (wsrc) f[i] = __fmul_rn(f[i], wf[i]);
+                    const double p = f0[i], q = f1[i];
+                    ss = fma(p, p, ss);
+                    st = fma(q, q, st);
                 }
-                if constexpr (!INTERLEAVED) {
-                    unpack8<BF16>(w_other, wf);
+                ss += st;
+#pragma unroll
+                for (int off = 1; off < kLanes; off <<= 1)
+                    ss += __shfl_xor_sync(0xffffffffu, ss, off);
+                if (kind != 2) {
+                    const float inv = rsqrt_rounded(ss * (1.0 / D) + a.eps);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        g[i] = __fmul_rn(g[i], inv);
-                        if (wsrc) g[i] = __fmul_rn(g[i], wf[i]);
+                        f0[i] = __fmul_rn(__fmul_rn(f0[i], inv), w0[i]);
+                        f1[i] = __fmul_rn(__fmul_rn(f1[i], inv), w1[i]);
                     }
-                }
-                if (rotates) {
                     if constexpr (INTERLEAVED) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float p = f[2 * i], s = f[2 * i + 1];
-                            f[2 * i] = __fsub_rn(__fmul_rn(p, cs[i].x), __fmul_rn(s, cs[i].y));
-                            f[2 * i + 1] = __fadd_rn(__fmul_rn(s, cs[i].x), __fmul_rn(p, cs[i].y));
+                        for (int i = 0; i < 8; ++i) {
+                            float* f = i < 4 ? f0 + 2 * i : f1 + 2 * (i - 4);
+                            if (!turns[i >> 2]) continue;
+                            const float p = f[0], q = f[1];
+                            f[0] = __fsub_rn(__fmul_rn(p, cs[i].x), __fmul_rn(q, cs[i].y));
+                            f[1] = __fadd_rn(__fmul_rn(q, cs[i].x), __fmul_rn(p, cs[i].y));
                         }
-                    } else {
+                    } else if (rotates) {
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
-                            const float own = __fmul_rn(f[i], cs[i].x);
-                            const float oth = __fmul_rn(g[i], cs[i].y);
-                            f[i] = second ? __fadd_rn(own, oth) : __fsub_rn(own, oth);
+                            const float p = f0[i], q = f1[i];
+                            f0[i] = __fsub_rn(__fmul_rn(p, cs[i].x), __fmul_rn(q, cs[i].y));
+                            f1[i] = __fadd_rn(__fmul_rn(q, cs[i].x), __fmul_rn(p, cs[i].y));
                         }
                     }
                 }
@@ -454,19 +507,49 @@ __global__ void __launch_bounds__(kInt4Threads) qk_norm_rope_kernel(RopeArgs a) 
                 if (store) {
                     uint16_t* out = kind == 0 ? a.q_out : a.k_out;
                     const long long row = (static_cast<long long>(b) * H + h) * a.T + t;
-                    reinterpret_cast<uint4*>(out)[row * kLPR + l] =
-                        make_uint4(pack2<BF16>(f[0], f[1]), pack2<BF16>(f[2], f[3]),
-                                   pack2<BF16>(f[4], f[5]), pack2<BF16>(f[6], f[7]));
+                    uint4* dst = reinterpret_cast<uint4*>(out) + row * (D / 8);
+                    dst[run0] = make_uint4(pack2<BF16>(f0[0], f0[1]), pack2<BF16>(f0[2], f0[3]),
+                                           pack2<BF16>(f0[4], f0[5]), pack2<BF16>(f0[6], f0[7]));
+                    dst[run1] = make_uint4(pack2<BF16>(f1[0], f1[1]), pack2<BF16>(f1[2], f1[3]),
+                                           pack2<BF16>(f1[4], f1[5]), pack2<BF16>(f1[6], f1[7]));
                 }
             }
             if constexpr (APPEND) {
+                if (!caches) continue;
+                if (!INTERLEAVED && a.rot != D) {
+                    // runs back into their natural order: run r is in lane `from`, first or second
+                    float n0[8], n1[8];
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+                        const int r = l + s * kLanes;
+                        int from = r;
+                        bool is_second = r >= kLanes;
+                        if (kind != 2) {
+                            const int tail = kLanes - rot_lanes;  // lanes behind the rotated part
+                            is_second = r < 2 * rot_lanes ? r >= rot_lanes : r - 2 * rot_lanes >= tail;
+                            from = r < 2 * rot_lanes ? (is_second ? r - rot_lanes : r)
+                                                     : r - rot_lanes - (is_second ? tail : 0);
+                        } else if (is_second) {
+                            from = r - kLanes;
+                        }
+                        from += lane - l;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float p = __shfl_sync(0xffffffffu, f0[i], from);
+                            const float q = __shfl_sync(0xffffffffu, f1[i], from);
+                            (s == 0 ? n0 : n1)[i] = is_second ? q : p;
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) f0[i] = n0[i], f1[i] = n1[i];
+                }
                 // lanes of q rows take part in the shuffles and store nothing
                 const long long pos =
                     static_cast<long long>(a.starts ? a.starts[b] : a.t0) + static_cast<int>(t);
                 const bool ok = store && kind != 0 && pos >= 0 && pos < a.S_cap;
                 const long long row = (static_cast<long long>(b) * a.Hkv + h) * a.S_cap + pos;
-                store_int4<D, BS>(f, l, row, ok, kind == 1 ? a.kc : a.vc,
-                                  kind == 1 ? a.kp : a.vp);
+                store_int4_runs<D, BS>(f0, f1, l, row, ok, kind == 1 ? a.kc : a.vc,
+                                       kind == 1 ? a.kp : a.vp);
             }
         }
     }

@@ -91,8 +91,9 @@ tqkv_status make_rows(Int4Rows& g, int B, int H, int T, int D, int S_cap, const 
 bool strides_ok(const long long* s) { return s[0] % 8 == 0 && s[1] % 8 == 0 && s[2] % 8 == 0; }
 
 struct DecodePlan4 {
-    int nt, rec_rows, slices, tile;
-    long long tiles;  // at most: every sequence S rows long
+    int nt, rec_rows, slices;
+    long long units, granules;  // granules at most: every sequence S rows long
+    long long tiles;
 };
 
 DecodePlan4 plan_int4(int B, int Hq, int Hkv, int S, int D) {
@@ -101,20 +102,31 @@ DecodePlan4 plan_int4(int B, int Hq, int Hkv, int S, int D) {
     p.nt = group > 8 ? 2 : 1;
     p.rec_rows = group < 8 * p.nt ? group : 8 * p.nt;
     p.slices = (group + 8 * p.nt - 1) / (8 * p.nt);
-    p.tile = 4096 / D;
-    p.tiles = static_cast<long long>(B) * Hkv * p.slices * ((static_cast<long long>(S) + p.tile - 1) / p.tile);
+    p.units = static_cast<long long>(B) * Hkv * p.slices;
+    p.granules = p.units * ((static_cast<long long>(S) + kGranule - 1) / kGranule);
+    p.tiles = p.granules / (4096 / D / kGranule);
     return p;
 }
 
-constexpr int kI4MaxCtasPerSm = 4;  // launch bounds of the decode kernel
-constexpr int kI4MinTiles = kI4Warps;
+// Warps a CTA.
+int int4_warps(const DecodePlan4& p, int sms) {
+    const int most = p.nt == 1 ? kI4MaxWarps : 8;
+    const int w = kI4MaxWarps;
+    return w < most ? w : most;
+}
 
-size_t int4_workspace(const DecodePlan4& p, int D, long long max_ctas) {
-    long long ctas = p.tiles / kI4MinTiles;
-    if (ctas > max_ctas) ctas = max_ctas;
-    if (ctas <= 1) return 0;
-    const size_t counters = (static_cast<size_t>(ctas) * 4 + 255) / 256 * 256;
-    return counters + static_cast<size_t>(ctas) * 2 * p.rec_rows * (D + 4) * sizeof(float);
+// Counters and two records for every CTA that the card can hold or the tiles can feed.
+long long int4_grid(const DecodePlan4& p, int warps, int sms) {
+    long long grid = p.tiles / warps;
+    const long long resident = static_cast<long long>(sms) * ((p.nt == 1 ? kI4MaxWarps : 8) / warps);
+    if (grid > resident) grid = resident;
+    return grid < 1 ? 1 : grid;
+}
+
+size_t int4_workspace(const DecodePlan4& p, int D, long long grid) {
+    if (grid <= 1) return 0;
+    return (static_cast<size_t>(grid) * 4 + 255) / 256 * 256 +
+           static_cast<size_t>(grid) * 2 * p.rec_rows * (D + 4) * sizeof(float);
 }
 
 template <int D, int BS, int NT>
@@ -125,32 +137,28 @@ tqkv_status decode_int4_impl(Int4DecodeArgs a, const DecodePlan4& p, int bf16, v
     cudaError_t e = current_sms(&dev, &sms);
     if (e != cudaSuccess) return from_cuda(e);
     auto fn = decode_int4_kernel<D, BS, NT>;
-    const int smem = C::smem_bytes(p.rec_rows);
-    // opt in and occupancy, once per device and record height
-    static std::atomic<int> known[kMaxDevices][C::kQ + 1];
-    int per_sm = known[dev][p.rec_rows].load(std::memory_order_acquire);
-    if (per_sm == 0) {
-        e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 C::smem_bytes(C::kQ));
-        if (e == cudaSuccess)
-            e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, fn, kI4Threads, smem);
+    constexpr int kSmem = 227 * 1024;
+    static std::atomic<bool> opted[kMaxDevices];
+    if (!opted[dev].load(std::memory_order_acquire)) {
+        e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
         if (e != cudaSuccess) return from_cuda(e);
-        if (per_sm < 1) return from_cuda(cudaErrorInvalidConfiguration);
-        if (per_sm > kI4MaxCtasPerSm) per_sm = kI4MaxCtasPerSm;
-        known[dev][p.rec_rows].store(per_sm, std::memory_order_release);
+        opted[dev].store(true, std::memory_order_release);
     }
-    long long grid = p.tiles / kI4MinTiles;
-    if (grid > static_cast<long long>(sms) * per_sm) grid = static_cast<long long>(sms) * per_sm;
-    if (grid < 1) grid = 1;
-    const size_t need = int4_workspace(p, D, static_cast<long long>(sms) * kI4MaxCtasPerSm);
-    if (grid > 1 && (!workspace || workspace_bytes < need)) return TQKV_ERR_WORKSPACE;
+    const int warps = int4_warps(p, sms);
+    long long grid = int4_grid(p, warps, sms);
+    if (grid > 1 && (!workspace || workspace_bytes < int4_workspace(p, D, grid)))
+        return TQKV_ERR_WORKSPACE;
+    // 1 KB of an SM's 228 KB of shared memory goes to each CTA besides its own
+    auto fit = [&](int stages) { return 228 * 1024 / (C::smem_bytes(warps, stages, p.rec_rows) + 1024); };
+    a.stages = fit(3) >= C::kWarps / warps ? 3 : 2;
+    if (fit(a.stages) < 1) return from_cuda(cudaErrorInvalidConfiguration);  // cannot happen
+    if (grid > static_cast<long long>(sms) * fit(a.stages)) grid = static_cast<long long>(sms) * fit(a.stages);
     if (!aligned(workspace, 16)) return TQKV_ERR_MISALIGNED;
     a.counters = static_cast<unsigned int*>(workspace);
     a.recs = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) +
                                       (static_cast<size_t>(grid) * 4 + 255) / 256 * 256);
-    a.min_tiles = kI4MinTiles;
-    return from_cuda(launch_kernel_dependent(fn, dim3(static_cast<unsigned>(grid)),
-                                             dim3(kI4Threads), smem, stream, a, bf16));
+    return from_cuda(launch_kernel_dependent(fn, dim3(static_cast<unsigned>(grid)), dim3(32 * warps),
+                                             C::smem_bytes(warps, a.stages, p.rec_rows), stream, a, bf16));
 }
 
 }  // namespace
@@ -215,8 +223,8 @@ size_t tqkv_decode_int4_workspace_bytes(int B, int H_q, int H_kv, int S, int D) 
         return 0;
     int dev = 0, sms = 0;
     if (current_sms(&dev, &sms) != cudaSuccess) return 0;
-    return int4_workspace(plan_int4(B, H_q, H_kv, S, D), D,
-                          static_cast<long long>(sms) * kI4MaxCtasPerSm);
+    const DecodePlan4 p = plan_int4(B, H_q, H_kv, S, D);
+    return int4_workspace(p, D, int4_grid(p, int4_warps(p, sms), sms));
 }
 
 tqkv_status tqkv_decode_int4(const void* q, const uint8_t* kq, const void* ks, const uint8_t* vq,
@@ -247,9 +255,9 @@ tqkv_status tqkv_decode_int4(const void* q, const uint8_t* kq, const void* ks, c
     a.S = S;
     a.score_scale = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(D)));
     const DecodePlan4 p = plan_int4(B, H_q, H_kv, S, D);
+    if (p.granules > INT_MAX) return TQKV_ERR_INVALID_SIZE;
     a.slices = p.slices;
     a.rec_rows = p.rec_rows;
-    a.stream_once = 1;
     const int bf16 = dtype == TQKV_BF16;
     return for_shape(D, block_size, [&](auto d, auto bs) {
         return p.nt == 1 ? decode_int4_impl<d(), bs(), 1>(a, p, bf16, workspace, workspace_bytes, stream)
@@ -321,9 +329,9 @@ static tqkv_status rope_checked(const tqkv_norm_rope_args* p, bool append, cudaS
     a.s3 = axes > 3 ? a.s2 + p->sections[2] : INT_MAX;
     const int kv_kinds = append ? 2 : 1;
     const long long rows = tokens * (p->H_q + static_cast<long long>(kv_kinds) * p->H_kv);
-    const int rows_per_cta = kInt4Threads / (D / 8);
+    const int rows_per_cta = kInt4Threads / (D / 16);
     // one head per lane group while that does not fill the card twice over; then several
-    a.heads_per_group = rows <= 16ll * sms * rows_per_cta ? 1 : 2 * kRopeUnroll;
+    a.heads_per_group = rows <= 16ll * sms * rows_per_cta ? 1 : 4 * kRopeUnroll;
     const int hpg = a.heads_per_group;
     a.q_groups = (p->H_q + hpg - 1) / hpg;
     a.kv_groups = (p->H_kv + hpg - 1) / hpg;

@@ -18,48 +18,45 @@ from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
-from ._lib import NormRopeArgs, check, load
+from ._lib import NormRopeArgs, TqkvError, check, load
 from .ops import Workspace
 
+_F16 = torch.float16
+_U8 = torch.uint8
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 _L3 = ctypes.c_longlong * 3
+_current_device = torch._C._cuda_getDevice
+_current_stream = torch._C._cuda_getCurrentRawStream
+
+# A decode step of a served model makes a few of these calls per layer, each
+# shorter on the GPU than a careless wrapper is on the host.  So the checks
+# below ask each tensor for as little as possible, once.
 
 
-class _Launch:
-    """The device and stream of a call: enters the device, gives the stream's handle, and tells
-    torch's allocator about tensors that another stream than the current one uses."""
+def _device(t: torch.Tensor, name: str) -> int:
+    """The index of t's CUDA device."""
+    index = t.get_device()
+    if index < 0:
+        raise ValueError(f"{name} must be on a CUDA device")
+    return index
 
-    __slots__ = ("guard", "handle", "other")
 
-    def __init__(self, device: torch.device, stream):
-        if device.type != "cuda":
-            raise ValueError("tensors must be on a CUDA device")
-        if stream is not None and stream.device != device:
-            raise ValueError(f"stream is on {stream.device}, tensors are on {device}")
-        self.guard = None if torch.cuda.current_device() == device.index \
-            else torch.cuda.device(device)
-        self.other = None
-        if stream is None:
-            self.handle = torch._C._cuda_getCurrentRawStream(device.index)
-        else:
-            self.handle = stream.cuda_stream
-            if self.handle != torch._C._cuda_getCurrentRawStream(device.index):
-                self.other = stream
+def _handle(index: int, stream) -> int:
+    """The stream to launch on, on device `index`."""
+    if stream is None:
+        return _current_stream(index)
+    if stream.device.index != index:
+        raise ValueError(f"stream is on {stream.device}, tensors are on cuda:{index}")
+    return stream.cuda_stream
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return self
 
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-
-    def used(self, *tensors) -> None:
-        if self.other is not None and not torch.cuda.is_current_stream_capturing():
-            for t in tensors:
-                if t is not None:
-                    t.record_stream(self.other)
+def _used(index: int, stream, *tensors) -> None:
+    """Tells torch's allocator about tensors that another stream than their own uses."""
+    if stream.cuda_stream != _current_stream(index) and \
+            not torch.cuda.is_current_stream_capturing():
+        for t in tensors:
+            if isinstance(t, torch.Tensor):
+                t.record_stream(stream)
 
 
 def _dtype(t: torch.Tensor, name: str) -> int:
@@ -69,57 +66,55 @@ def _dtype(t: torch.Tensor, name: str) -> int:
     return code
 
 
-def _is(t: Optional[torch.Tensor], name: str, shape: tuple, dtype: torch.dtype,
-        device: torch.device) -> int:
+def _is(t: Optional[torch.Tensor], name: str, shape: tuple, dtype: torch.dtype, index: int) -> int:
     """The address of a contiguous tensor of exactly this shape, type and device."""
     if t is None:
         raise ValueError(f"{name} is required")
-    if t.shape != shape or t.dtype != dtype or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor {shape} on {device}, got "
-                         f"{t.dtype} {tuple(t.shape)} on {t.device}")
+    if t.dtype is not dtype or t.get_device() != index or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor {tuple(shape)} on "
+                         f"cuda:{index}, got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-def _rows(x: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device):
+def _rows(x: torch.Tensor, name: str, dtype: torch.dtype, index: int):
     """(shape, strides of the first three dimensions) of x [B, H, T, D]."""
-    if x.dim() != 4 or x.dtype != dtype or x.device != device:
-        raise ValueError(f"{name} must be a {dtype} tensor [B, H, T, D] on {device}, got "
+    if x.dtype is not dtype or x.get_device() != index or x.dim() != 4:
+        raise ValueError(f"{name} must be a {dtype} tensor [B, H, T, D] on cuda:{index}, got "
                          f"{x.dtype} {tuple(x.shape)} on {x.device}")
-    shape, st = x.shape, x.stride()
-    if st[3] != 1 and shape[3] != 1:
+    shape = x.shape
+    sb, sh, st, sd = x.stride()
+    if sd != 1 and shape[3] != 1:
         raise ValueError(f"{name}: the last dimension must be adjacent in memory")
-    # the stride of a dimension of one element means nothing
-    strides = tuple(0 if n == 1 else s for n, s in zip(shape[:3], st))
-    if strides[0] % 8 or strides[1] % 8 or strides[2] % 8:
-        raise ValueError(f"{name}: strides must be multiples of 8 elements, got {tuple(st)}")
-    return shape, strides
+    if (sb | sh | st) & 7:
+        # the stride of a dimension of one element means nothing
+        sb, sh, st = (0 if n == 1 else s for n, s in zip(shape, (sb, sh, st)))
+        if (sb | sh | st) & 7:
+            raise ValueError(f"{name}: strides must be multiples of 8 elements, got {x.stride()}")
+    return shape, (sb, sh, st)
 
 
-def _cache(q: torch.Tensor, s: torch.Tensor, qn: str, sn: str, block_size: int,
-           device: torch.device) -> Tuple[int, int, int, int]:
-    """(B, H, S_cap, D) of a cache's codes and scales."""
-    if q.dim() != 4:
-        raise ValueError(f"{qn} must be uint8 [B, H, S_cap, D // 2]")
-    B, H, S, half = q.shape
-    _is(q, qn, (B, H, S, half), torch.uint8, device)
+def _cache(q: torch.Tensor, s: torch.Tensor, qn: str, sn: str, block_size: int, index: int):
+    """(codes' shape, D, scales' shape) of a cache."""
+    if q.dtype is not _U8 or q.get_device() != index or q.dim() != 4 or not q.is_contiguous():
+        raise ValueError(f"{qn} must be a contiguous uint8 tensor [B, H, S_cap, D // 2] on "
+                         f"cuda:{index}, got {q.dtype} {tuple(q.shape)} on {q.device}")
+    shape = q.shape
+    B, H, S, half = shape
     D = 2 * half
     if block_size <= 0 or D % block_size:
         raise ValueError(f"block_size {block_size} does not divide D {D}")
-    _is(s, sn, (B, H, S, D // block_size, 2), torch.float16, device)
-    return B, H, S, D
+    if S > 0x7fffffff:
+        raise ValueError(f"S_cap {S} does not fit 32 bits")
+    params = (B, H, S, D // block_size, 2)
+    _is(s, sn, params, _F16, index)
+    return shape, D, params
 
 
-def _starts(t0: Union[int, torch.Tensor], B: int, device: torch.device):
+def _starts(t0: Union[int, torch.Tensor], B: int, index: int):
     """(address of the per-sequence first rows or None, first row of all)."""
     if isinstance(t0, torch.Tensor):
-        return _is(t0, "t0", (B,), torch.int32, device), 0
-    return None, int(t0)
-
-
-def _bound(**sizes: int) -> None:
-    for name, n in sizes.items():
-        if n > 0x7fffffff:
-            raise ValueError(f"{name} = {n} does not fit 32 bits")
+        return _is(t0, "t0", (B,), torch.int32, index), 0
+    return None, t0
 
 
 def kv_compress_int4(x: torch.Tensor, block_size: int, xq: Optional[torch.Tensor] = None,
@@ -134,7 +129,9 @@ def kv_compress_int4(x: torch.Tensor, block_size: int, xq: Optional[torch.Tensor
     if xq is None:
         xq = torch.empty((B, H, S, D // 2), dtype=torch.uint8, device=x.device)
     if scales is None:
-        scales = torch.empty((B, H, S, D // block_size, 2), dtype=torch.float16, device=x.device)
+        scales = torch.empty((B, H, S, D // block_size, 2), dtype=_F16, device=x.device)
+    if xq.dim() != 4 or xq.shape[2] != S:
+        raise ValueError(f"xq {tuple(xq.shape)} does not have x's {S} rows")
     kv_append_int4(x, xq, scales, 0, block_size, stream=stream)
     return xq, scales
 
@@ -142,19 +139,23 @@ def kv_compress_int4(x: torch.Tensor, block_size: int, xq: Optional[torch.Tensor
 def kv_append_int4(x: torch.Tensor, cache_q: torch.Tensor, cache_s: torch.Tensor,
                    t0: Union[int, torch.Tensor], block_size: int, stream=None) -> None:
     """Quantise T tokens per head, x [B, H, T, D], into rows [t0, t0 + T) of a 4-bit cache."""
-    device = x.device
+    index = _device(x, "x")
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return kv_append_int4(x, cache_q, cache_s, t0, block_size, stream)
     dt = _dtype(x, "x")
-    shape, strides = _rows(x, "x", x.dtype, device)
-    B, H, S_cap, D = _cache(cache_q, cache_s, "cache_q", "cache_s", block_size, device)
-    if (B, H, D) != (shape[0], shape[1], shape[3]):
-        raise ValueError(f"cache_q {tuple(cache_q.shape)} does not match x {tuple(shape)}")
-    _bound(S_cap=S_cap)
-    starts, first = _starts(t0, B, device)
-    with _Launch(device, stream) as on:
-        check("tqkv_kv_append_int4", load().tqkv_kv_append_int4(
-            x.data_ptr(), _L3(*strides), cache_q.data_ptr(), cache_s.data_ptr(), starts, first,
-            B, H, shape[2], D, block_size, S_cap, dt, on.handle))
-        on.used(x, cache_q, cache_s, t0 if starts else None)
+    (Bx, Hx, T, Dx), strides = _rows(x, "x", x.dtype, index)
+    (B, H, S_cap, _), D, _ = _cache(cache_q, cache_s, "cache_q", "cache_s", block_size, index)
+    if B != Bx or H != Hx or D != Dx:
+        raise ValueError(f"cache_q {tuple(cache_q.shape)} does not match x {tuple(x.shape)}")
+    starts, first = _starts(t0, B, index)
+    status = load().tqkv_kv_append_int4(
+        x.data_ptr(), _L3(*strides), cache_q.data_ptr(), cache_s.data_ptr(), starts, first, B, H, T,
+        D, block_size, S_cap, dt, _handle(index, stream))
+    if status:
+        raise TqkvError("tqkv_kv_append_int4", status)
+    if stream is not None:
+        _used(index, stream, x, cache_q, cache_s, t0)
 
 
 def kv_reconstruct_int4(xq: torch.Tensor, scales: torch.Tensor, block_size: int,
@@ -163,23 +164,31 @@ def kv_reconstruct_int4(xq: torch.Tensor, scales: torch.Tensor, block_size: int,
                         stream=None) -> torch.Tensor:
     """The values of rows [t0, t0 + T) of a 4-bit cache (all of them by default): [B, H, T, D] in
     `dtype`, or in y's."""
-    device = xq.device
-    B, H, S_cap, D = _cache(xq, scales, "xq", "scales", block_size, device)
+    index = _device(xq, "xq")
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return kv_reconstruct_int4(xq, scales, block_size, y, t0, T, dtype, stream)
+    (B, H, S_cap, _), D, _ = _cache(xq, scales, "xq", "scales", block_size, index)
+    starts, first = _starts(t0, B, index)
     if T is None:
-        if isinstance(t0, torch.Tensor):
+        if starts is not None:
             raise ValueError("T is required with a tensor t0")
-        T = S_cap - t0
-    _bound(S_cap=S_cap)
-    starts, first = _starts(t0, B, device)
-    with _Launch(device, stream) as on:
-        if y is None:
-            y = torch.empty((B, H, max(T, 0), D), dtype=dtype, device=device)
+        T = S_cap - first
+    if y is None:
+        # scales is fp16 on the right device: the cheapest way to a tensor like it
+        y = scales.new_empty((B, H, T if T > 0 else 0, D)) if dtype is _F16 else \
+            scales.new_empty((B, H, T if T > 0 else 0, D), dtype=dtype)
+        dt = _dtype(y, "dtype")
+    else:
         dt = _dtype(y, "y")
-        _is(y, "y", (B, H, T, D), y.dtype, device)
-        check("tqkv_kv_reconstruct_int4", load().tqkv_kv_reconstruct_int4(
-            xq.data_ptr(), scales.data_ptr(), y.data_ptr(), starts, first, B, H, T, D, block_size,
-            S_cap, dt, on.handle))
-        on.used(xq, scales, y, t0 if starts else None)
+        _is(y, "y", (B, H, T, D), y.dtype, index)
+    status = load().tqkv_kv_reconstruct_int4(
+        xq.data_ptr(), scales.data_ptr(), y.data_ptr(), starts, first, B, H, T, D, block_size,
+        S_cap, dt, _handle(index, stream))
+    if status:
+        raise TqkvError("tqkv_kv_reconstruct_int4", status)
+    if stream is not None:
+        _used(index, stream, xq, scales, y, t0)
     return y
 
 
@@ -187,33 +196,35 @@ _default_ws: dict = {}
 _ws_bytes: dict = {}
 
 
-def _workspace(ws: Optional[Workspace], device: torch.device, handle: int, stream, key):
+def _workspace(ws: Optional[Workspace], index: int, handle: int, stream, key):
     """(address, bytes, tensor to keep) of the scratch for a decode of sizes `key`.  Without a
     Workspace of the caller's, every stream has its own; a call that is being captured gets its own
     buffer from the graph's memory, zeroed by the graph, so that graphs may replay side by side."""
-    need = _ws_bytes.get((device.index, key))
+    need = _ws_bytes.get((index, key))
     if need is None:
         need = int(load().tqkv_decode_int4_workspace_bytes(*key))
         if len(_ws_bytes) < 4096:
-            _ws_bytes[(device.index, key)] = need
+            _ws_bytes[(index, key)] = need
     if need == 0:
         return None, 0, None
-    if ws is not None and ws.device.index not in (None, device.index):
-        raise ValueError(f"workspace is on {ws.device}, tensors are on {device}")
-    big_enough = ws is not None and ws.buf is not None and ws.buf.numel() >= need
-    if big_enough:
-        return ws.buf.data_ptr(), ws.buf.numel(), ws.buf
+    if ws is not None:
+        if ws.device.index not in (None, index):
+            raise ValueError(f"workspace is on {ws.device}, tensors are on cuda:{index}")
+        if ws.buf is not None and ws.buf.numel() >= need:
+            return ws.buf.data_ptr(), ws.buf.numel(), ws.buf
     if torch.cuda.is_current_stream_capturing():
         if ws is not None:
             raise ValueError("a Workspace cannot grow while a graph is captured: call once before "
                              "the capture, or leave the workspace to the call")
-        buf = torch.empty(need, dtype=torch.uint8, device=device)
-        check("tqkv_workspace_init", load().tqkv_workspace_init(buf.data_ptr(), need, handle))
+        buf = torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", index))
+        # only the counters in front (4 bytes a CTA) have to be zero: no INT8 call uses this buffer
+        check("tqkv_workspace_init",
+              load().tqkv_workspace_init(buf.data_ptr(), min(need, 16384), handle))
         return buf.data_ptr(), need, buf
     if ws is None:
-        ws = _default_ws.get((device.index, handle))
+        ws = _default_ws.get((index, handle))
         if ws is None:
-            ws = _default_ws[(device.index, handle)] = Workspace(device)
+            ws = _default_ws[(index, handle)] = Workspace(torch.device("cuda", index))
     ptr, size = ws.get(need, stream)
     return ptr, size, ws.buf
 
@@ -227,31 +238,39 @@ def decode_int4(q: torch.Tensor, kq: torch.Tensor, ks: torch.Tensor, vq: torch.T
     q [B, H_q, D]; caches with H_kv heads, H_q a multiple of H_kv.  Sequence b attends over its
     first lengths[b] rows (int32 [B] on the device, taken into [0, S]), or over S rows; S defaults
     to the cache's.  A sequence without rows gives zeros."""
-    device = q.device
+    index = _device(q, "q")
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return decode_int4(q, kq, ks, vq, vs, block_size, S, lengths, out, workspace, stream)
     dt = _dtype(q, "q")
+    shape, D, params = _cache(kq, ks, "kq", "ks", block_size, index)
+    B, H_kv, S_cap, _ = shape
+    v_ptr = _is(vq, "vq", shape, _U8, index)
+    vs_ptr = _is(vs, "vs", params, _F16, index)
     if q.dim() != 3:
         raise ValueError("q must be [B, H_q, D]")
-    B, H_kv, S_cap, D = _cache(kq, ks, "kq", "ks", block_size, device)
-    _is(vq, "vq", kq.shape, torch.uint8, device)
-    _is(vs, "vs", ks.shape, torch.float16, device)
     H_q = q.shape[1]
-    _is(q, "q", (B, H_q, D), q.dtype, device)
+    q_ptr = _is(q, "q", (B, H_q, D), q.dtype, index)
     if S is None:
         S = S_cap
-    _bound(S_cap=S_cap, S=S)
+    elif S > 0x7fffffff:
+        raise ValueError(f"S {S} does not fit 32 bits")
     if H_kv == 0 or H_q % H_kv:
         raise ValueError(f"H_q {H_q} is not a multiple of H_kv {H_kv}")
-    n = None if lengths is None else _is(lengths, "lengths", (B,), torch.int32, device)
-    with _Launch(device, stream) as on:
-        if out is None:
-            out = torch.empty((B, H_q, D), dtype=q.dtype, device=device)
-        else:
-            _is(out, "out", (B, H_q, D), q.dtype, device)
-        ptr, size, buf = _workspace(workspace, device, on.handle, stream, (B, H_q, H_kv, S, D))
-        check("tqkv_decode_int4", load().tqkv_decode_int4(
-            q.data_ptr(), kq.data_ptr(), ks.data_ptr(), vq.data_ptr(), vs.data_ptr(), n,
-            out.data_ptr(), B, H_q, H_kv, S, S_cap, D, block_size, dt, ptr, size, on.handle))
-        on.used(q, kq, ks, vq, vs, lengths, out, buf)
+    n = None if lengths is None else _is(lengths, "lengths", (B,), torch.int32, index)
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        _is(out, "out", (B, H_q, D), q.dtype, index)
+    handle = _handle(index, stream)
+    ptr, size, buf = _workspace(workspace, index, handle, stream, (B, H_q, H_kv, S, D))
+    status = load().tqkv_decode_int4(
+        q_ptr, kq.data_ptr(), ks.data_ptr(), v_ptr, vs_ptr, n, out.data_ptr(), B, H_q, H_kv, S,
+        S_cap, D, block_size, dt, ptr, size, handle)
+    if status:
+        raise TqkvError("tqkv_decode_int4", status)
+    if stream is not None:
+        _used(index, stream, q, kq, ks, vq, vs, lengths, out, buf)
     return out
 
 
@@ -267,38 +286,46 @@ def rope_table(max_pos: int, rot_dim: int, base: float = 10000.0, device=None) -
     return torch.stack((angle.cos(), angle.sin()), -1).float()
 
 
-def _norm_rope(q, k, positions, table, q_weight, k_weight, eps, interleaved, sections):
-    """The arguments that both forms share, and (B, H_q, H_kv, T, D)."""
-    device = q.device
+def _norm_rope(index, q, k, positions, table, q_weight, k_weight, eps, interleaved, sections):
+    """The arguments that both forms share, and k's shape."""
     a = NormRopeArgs()
     a.dtype = _dtype(q, "q")
-    (B, H_q, T, D), qs = _rows(q, "q", q.dtype, device)
-    (Bk, H_kv, Tk, Dk), kst = _rows(k, "k", q.dtype, device)
-    if (Bk, Tk, Dk) != (B, T, D):
+    dtype = q.dtype
+    (B, H_q, T, D), qs = _rows(q, "q", dtype, index)
+    k_shape, kst = _rows(k, "k", dtype, index)
+    Bk, H_kv, Tk, Dk = k_shape
+    if Bk != B or Tk != T or Dk != D:
         raise ValueError(f"k {tuple(k.shape)} does not match q {tuple(q.shape)}")
     if table.dim() != 3:
         raise ValueError("table must be float32 [max_pos, rot_dim // 2, 2]")
-    max_pos, pairs = table.shape[0], table.shape[1]
-    a.table = _is(table, "table", (max_pos, pairs, 2), torch.float32, device)
+    max_pos, pairs, _ = table.shape
+    a.table = _is(table, "table", (max_pos, pairs, 2), torch.float32, index)
     if sections is None:
-        axes = 1
-        a.positions = _is(positions, "positions", (B, T), torch.int32, device)
+        a.axes = 1
+        a.positions = _is(positions, "positions", (B, T), torch.int32, index)
     else:
-        axes = len(sections)
+        axes = a.axes = len(sections)
         if not 1 <= axes <= 4 or sum(sections) != pairs or min(sections) < 0:
             raise ValueError(f"sections {tuple(sections)}: 1 to 4 counts that sum to {pairs}")
-        a.positions = _is(positions, "positions", (axes, B, T), torch.int32, device)
-        a.sections[:axes] = list(sections)
-    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        if w is not None:
-            setattr(a, name, _is(w, name, (D,), q.dtype, device))
-    _bound(max_pos=max_pos)
+        a.positions = _is(positions, "positions", (axes, B, T), torch.int32, index)
+        a.sections[:axes] = sections
+    if q_weight is not None:
+        a.q_weight = _is(q_weight, "q_weight", (D,), dtype, index)
+    if k_weight is not None:
+        a.k_weight = _is(k_weight, "k_weight", (D,), dtype, index)
+    if max_pos > 0x7fffffff:
+        raise ValueError(f"max_pos {max_pos} does not fit 32 bits")
     a.q, a.k = q.data_ptr(), k.data_ptr()
     a.q_strides[:], a.k_strides[:] = qs, kst
     a.eps = eps
     a.B, a.H_q, a.H_kv, a.T, a.D = B, H_q, H_kv, T, D
-    a.rot_dim, a.max_pos, a.interleaved, a.axes = 2 * pairs, max_pos, bool(interleaved), axes
-    return a, (B, H_q, H_kv, T, D)
+    a.rot_dim, a.max_pos, a.interleaved = 2 * pairs, max_pos, bool(interleaved)
+    return a, k_shape
+
+
+def _new_rows(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of t's shape, type and device."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table: torch.Tensor,
@@ -313,19 +340,27 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, tabl
     rot_dim = 2 * table.shape[1] elements becomes (a cos - b sin, b cos + a sin).  Pairs are (j, j +
     rot_dim / 2), or (2 j, 2 j + 1) if `interleaved`.  positions: int32 [B, T], or [axes, B, T] with
     `sections`, the number of pairs that follow each axis.  A position outside the table gives
-    NaN."""
-    device = q.device
-    a, (B, H_q, H_kv, T, D) = _norm_rope(q, k, positions, table, q_weight, k_weight, eps,
-                                         interleaved, sections)
-    with _Launch(device, stream) as on:
-        if q_out is None:
-            q_out = torch.empty((B, H_q, T, D), dtype=q.dtype, device=device)
-        if k_out is None:
-            k_out = torch.empty((B, H_kv, T, D), dtype=q.dtype, device=device)
-        a.q_out = _is(q_out, "q_out", (B, H_q, T, D), q.dtype, device)
-        a.k_out = _is(k_out, "k_out", (B, H_kv, T, D), q.dtype, device)
-        check("tqkv_qk_norm_rope", load().tqkv_qk_norm_rope(ctypes.byref(a), on.handle))
-        on.used(q, k, positions, table, q_weight, k_weight, q_out, k_out)
+    NaN.  Outputs must not overlap the inputs."""
+    index = _device(q, "q")
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return qk_norm_rope(q, k, positions, table, q_weight, k_weight, eps, interleaved,
+                                sections, q_out, k_out, stream)
+    a, _ = _norm_rope(index, q, k, positions, table, q_weight, k_weight, eps, interleaved, sections)
+    if q_out is None:
+        q_out = _new_rows(q)
+    else:
+        _is(q_out, "q_out", q.shape, q.dtype, index)
+    if k_out is None:
+        k_out = _new_rows(k)
+    else:
+        _is(k_out, "k_out", k.shape, q.dtype, index)
+    a.q_out, a.k_out = q_out.data_ptr(), k_out.data_ptr()
+    status = load().tqkv_qk_norm_rope(ctypes.byref(a), _handle(index, stream))
+    if status:
+        raise TqkvError("tqkv_qk_norm_rope", status)
+    if stream is not None:
+        _used(index, stream, q, k, positions, table, q_weight, k_weight, q_out, k_out)
     return q_out, k_out
 
 
@@ -340,29 +375,37 @@ def qk_norm_rope_append_int4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     """qk_norm_rope with K and V [B, H_kv, T, D] written straight into rows [t0, t0 + T) of their
     4-bit caches, in one launch; returns q [B, H_q, T, D].  K is quantised from fp32, without the
     rounding to its type that qk_norm_rope followed by kv_append_int4 has."""
-    device = q.device
-    a, (B, H_q, H_kv, T, D) = _norm_rope(q, k, positions, table, q_weight, k_weight, eps,
-                                         interleaved, sections)
-    shape, vst = _rows(v, "v", q.dtype, device)
-    if shape != k.shape:
-        raise ValueError(f"v {tuple(shape)} does not match k {tuple(k.shape)}")
-    Bc, Hc, S_cap, Dc = _cache(kq, ks, "kq", "ks", block_size, device)
-    if (Bc, Hc, Dc) != (B, H_kv, D):
+    index = _device(q, "q")
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return qk_norm_rope_append_int4(q, k, v, positions, table, kq, ks, vq, vs, t0,
+                                            block_size, q_weight, k_weight, eps, interleaved,
+                                            sections, q_out, stream)
+    a, k_shape = _norm_rope(index, q, k, positions, table, q_weight, k_weight, eps, interleaved,
+                            sections)
+    v_shape, vst = _rows(v, "v", q.dtype, index)
+    if v_shape != k_shape:
+        raise ValueError(f"v {tuple(v_shape)} does not match k {tuple(k_shape)}")
+    shape, D, params = _cache(kq, ks, "kq", "ks", block_size, index)
+    B, H_kv, S_cap, _ = shape
+    if (B, H_kv, D) != (k_shape[0], k_shape[1], k_shape[3]):
         raise ValueError(f"kq {tuple(kq.shape)} does not match k {tuple(k.shape)}")
-    _is(vq, "vq", kq.shape, torch.uint8, device)
-    _is(vs, "vs", ks.shape, torch.float16, device)
-    _bound(S_cap=S_cap)
-    starts, a.t0 = _starts(t0, B, device)
-    a.starts = starts
-    a.v, a.v_strides[:] = v.data_ptr(), vst
-    a.kq, a.ks, a.vq, a.vs = kq.data_ptr(), ks.data_ptr(), vq.data_ptr(), vs.data_ptr()
+    a.vq = _is(vq, "vq", shape, _U8, index)
+    a.vs = _is(vs, "vs", params, _F16, index)
+    a.starts, a.t0 = _starts(t0, B, index)
+    a.v = v.data_ptr()
+    a.v_strides[:] = vst
+    a.kq, a.ks = kq.data_ptr(), ks.data_ptr()
     a.block_size, a.S_cap = block_size, S_cap
-    with _Launch(device, stream) as on:
-        if q_out is None:
-            q_out = torch.empty((B, H_q, T, D), dtype=q.dtype, device=device)
-        a.q_out = _is(q_out, "q_out", (B, H_q, T, D), q.dtype, device)
-        check("tqkv_qk_norm_rope_append_int4",
-              load().tqkv_qk_norm_rope_append_int4(ctypes.byref(a), on.handle))
-        on.used(q, k, v, positions, table, kq, ks, vq, vs, t0 if starts else None, q_weight,
-                k_weight, q_out)
+    if q_out is None:
+        q_out = _new_rows(q)
+    else:
+        _is(q_out, "q_out", q.shape, q.dtype, index)
+    a.q_out = q_out.data_ptr()
+    status = load().tqkv_qk_norm_rope_append_int4(ctypes.byref(a), _handle(index, stream))
+    if status:
+        raise TqkvError("tqkv_qk_norm_rope_append_int4", status)
+    if stream is not None:
+        _used(index, stream, q, k, v, positions, table, kq, ks, vq, vs, t0, q_weight, k_weight,
+              q_out)
     return q_out
