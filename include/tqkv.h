@@ -429,7 +429,7 @@ typedef struct tqkv_norm_rope_args {
     long long v_strides[3];
     const void* q_weight;     /* [D], or null for 1 */
     const void* k_weight;
-    const float* table;       /* [max_pos, rot_dim / 2, 2], 8-byte aligned */
+    const float* table;       /* [max_pos, rot_dim / 2, 2] */
     const int32_t* positions; /* device, [axes, B, T] */
     void* q_out;              /* [B, H_q, T, D] */
     void* k_out;              /* [B, H_kv, T, D]; unused by the append */

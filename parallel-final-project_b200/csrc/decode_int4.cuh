@@ -145,24 +145,6 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
     return d;
 }
 
-// `bytes` (4, 8 or 16) of global memory into shared memory, or zeros
-template <int bytes>
-__device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool real = true) {
-    if constexpr (bytes == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
-                     "r"(real ? 16 : 0)
-                     : "memory");
-    else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src),
-                     "n"(bytes), "r"(real ? bytes : 0)
-                     : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 // N words from shared memory by one load
 template <int N>
 __device__ __forceinline__ void lds_words(uint32_t (&w)[N], const uint8_t* p) {

@@ -19,12 +19,14 @@
 // and a decode lane that loads them with one instruction can still apply a
 // scale per group (decode_int4.cuh).
 //
-// Bound: HBM.  One lane owns 8 elements (one 16-byte load), D / 8 lanes a row.
+// Bound: HBM, with the issue slots close behind; so a lane owns 16 elements,
+// D / 16 lanes a row, which halves what every lane does once per row and block.
 #pragma once
 
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <type_traits>
 
 #include "device_common.cuh"
 #include "kv_compress.cuh"
@@ -44,6 +46,24 @@ struct FastDiv {
         return (__umulhi(n, m) + n) >> s;
     }
 };
+
+// `bytes` (4, 8 or 16) of global memory into shared memory, or zeros
+template <int bytes>
+__device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool real = true) {
+    if constexpr (bytes == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+                     "r"(real ? 16 : 0)
+                     : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src),
+                     "n"(bytes), "r"(real ? bytes : 0)
+                     : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 
 // max / min that keep a NaN operand
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -84,78 +104,63 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     }
 }
 
-// Codes of one lane's 8 values, given its block's minimum and maximum; sets
-// `params` to the block's (scale, zero).
-//
+// What a block's codes are made with.
+struct BlockScale {
+    float zero, r, e;  // 1 / (16 scale) = r + e
+    uint32_t params;   // (scale, zero) as stored
+};
+
 // The quotient d / scale decides a code by its distance from a half-integer,
 // and fp16 inputs do meet half-integers exactly, where a reciprocal rounded to
 // 24 bits would fall to either side.  So the reciprocal is carried in two
 // words, r + e with e = (1 - scale * r) * r: d * r + d * e has a relative
-// error below 2^-45 before its one rounding, which returns an exact
+// error below 2^-43 before its one rounding, which returns an exact
 // half-integer quotient as that half-integer.  One multiply and one FMA an
-// element instead of a division.
-__device__ __forceinline__ uint32_t int4_codes(const float (&f)[8], float lo, float hi,
-                                               uint32_t& params) {
+// element instead of a division.  Division by 15 likewise: a quotient by 15
+// lies at least 1 / 30 of a step from the middle between two fp32 values, so
+// its rounding is the division's.
+__device__ __forceinline__ BlockScale block_scale(float lo, float hi) {
+    constexpr float k15 = 1.0f / 15.0f;
+    constexpr float k15low = static_cast<float>(1.0 / 15.0 - static_cast<double>(k15));
+    const float range = hi - lo;
     __half zero = __float2half_rn(lo);
-    __half scale = __float2half_rn(__fdiv_rn(hi - lo, 15.0f));
-    float z = __half2float(zero);
-    float s = __half2float(scale);
-    float r = 0.0f, e = 0.0f;
-    if (!(fabsf(s) < INFINITY && fabsf(z) < INFINITY)) {
+    __half scale = __float2half_rn(fmaf(range, k15, range * k15low));
+    const float s = __half2float(scale);
+    BlockScale b;
+    b.zero = __half2float(zero);
+    b.r = b.e = 0.0f;
+    if (!(fabsf(s) < INFINITY && fabsf(b.zero) < INFINITY)) {
         zero = scale = __ushort_as_half(0x7fff);
     } else if (s > 0.0f) {
-        r = __frcp_rn(s);
-        e = fmaf(-s, r, 1.0f) * r;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(b.r) : "f"(s));
+        b.e = fmaf(-s, b.r, 1.0f) * b.r * 0.0625f;
+        b.r *= 0.0625f;
     }
-    params = __half_as_ushort(scale) | (static_cast<uint32_t>(__half_as_ushort(zero)) << 16);
-    // 1.5 * 2^23 + q rounds q to an integer, ties to even, in the low bits;
-    // fmaxf(NaN, 0) = 0 covers the blocks with r = 0 and infinite elements
-    constexpr float kMagic = 12582912.0f;
+    b.params = __half_as_ushort(scale) | (static_cast<uint32_t>(__half_as_ushort(zero)) << 16);
+    return b;
+}
+
+// One word of codes.  A quotient over 16 is clamped to [0, 1] by the FMA's
+// saturation, which also turns NaN to 0 (a block with r = 0 whose elements are
+// infinite), and to 15 / 16; 1.5 * 2^23 + 16 t then rounds it to an integer,
+// ties to even, in the low bits.  The words' sum of 16^i times those floats'
+// bits differs from the codes' by a constant.
+__device__ __forceinline__ uint32_t int4_codes(const float* f, const BlockScale& b) {
+    constexpr float kMagic = 12582912.0f;  // bits 0x4b400000
     uint32_t word = 0;
 #pragma unroll
     for (int i = 7; i >= 0; --i) {
-        const float d = f[i] - z;
-        const float q = fminf(fmaxf(fmaf(d, r, d * e), 0.0f), 15.0f);
-        word = (word << 4) | (__float_as_uint(q + kMagic) & 15u);
+        const float d = f[i] - b.zero;
+        const float t = fminf(__saturatef(fmaf(d, b.r, d * b.e)), 0.9375f);
+        word = word * 16u + __float_as_uint(fmaf(t, 16.0f, kMagic));
     }
-    return word;
-}
-
-// Minimum and maximum over the lane's block (aligned groups of BS / 8 lanes).
-template <int BS>
-__device__ __forceinline__ void block_range(const float (&f)[8], float& lo, float& hi) {
-    lo = hi = f[0];
-#pragma unroll
-    for (int i = 1; i < 8; ++i) {
-        lo = min_nan(lo, f[i]);
-        hi = max_nan(hi, f[i]);
-    }
-#pragma unroll
-    for (int off = 1; off < BS / 8; off <<= 1) {
-        lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, off));
-        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, off));
-    }
+    return word - 0x4b400000u * 0x11111111u;
 }
 
 // Where lane l's word stands in a packed row.
 template <int D>
 __device__ __forceinline__ int word_of_lane(int l) {
     return (l & 3) * (D / 32) + (l >> 2);
-}
-
-// Quantises lane l's 8 values of a row into the cache row `row`.  Every lane
-// of the warp calls it; rows with `valid` false are computed and dropped.
-template <int D, int BS>
-__device__ __forceinline__ void store_int4(const float (&f)[8], int l, long long row, bool valid,
-                                           uint32_t* __restrict__ codes,
-                                           uint32_t* __restrict__ params) {
-    float lo, hi;
-    block_range<BS>(f, lo, hi);
-    uint32_t p;
-    const uint32_t w = int4_codes(f, lo, hi, p);
-    if (!valid) return;
-    codes[row * (D / 8) + word_of_lane<D>(l)] = w;
-    if (l % (BS / 8) == 0) params[row * (D / BS) + l / (BS / 8)] = p;
 }
 
 // Rows [start_b, start_b + T) of every head of a cache, or of x.
@@ -182,36 +187,107 @@ struct Int4Rows {
 };
 
 constexpr int kInt4Threads = 256;
-constexpr int kInt4Unroll = 4;  // rows a lane keeps in flight
+constexpr int kInt4Unroll = 2;  // rows a lane keeps in flight, 32 bytes of each
+constexpr int kReadUnroll = 4;  // and 8 bytes of each when it reads back
+
+// Packed maximum of 16-bit pairs, NaN if either is.
+template <bool BF16>
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
+    if constexpr (BF16) {
+        const __nv_bfloat162 v = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&a),
+                                             *reinterpret_cast<const __nv_bfloat162*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&v);
+    } else {
+        const __half2 v = __hmax2_nan(*reinterpret_cast<const __half2*>(&a),
+                                      *reinterpret_cast<const __half2*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t min2_nan(uint32_t a, uint32_t b) {
+    if constexpr (BF16) {
+        const __nv_bfloat162 v = __hmin2_nan(*reinterpret_cast<const __nv_bfloat162*>(&a),
+                                             *reinterpret_cast<const __nv_bfloat162*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&v);
+    } else {
+        const __half2 v = __hmin2_nan(*reinterpret_cast<const __half2*>(&a),
+                                      *reinterpret_cast<const __half2*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+}
+
+// Range of the block that the lane's 16 elements belong to (aligned groups of
+// BS / 16 lanes): maximum and negated minimum go through one reduction.
+template <int BS, bool BF16>
+__device__ __forceinline__ void block_range16(const uint32_t (&w)[8], float& lo, float& hi) {
+    uint32_t mx = w[0], mn = w[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+        mx = max2_nan<BF16>(mx, w[i]);
+        mn = min2_nan<BF16>(mn, w[i]);
+    }
+    mn ^= 0x80008000u;
+    // (largest of the even, negated smallest of the even) and the same of the odd elements
+    uint32_t m = max2_nan<BF16>(__byte_perm(mx, mn, 0x5410), __byte_perm(mx, mn, 0x7632));
+#pragma unroll
+    for (int off = 1; off < BS / 16; off <<= 1)
+        m = max2_nan<BF16>(m, __shfl_xor_sync(0xffffffffu, m, off));
+    if constexpr (BF16) {
+        hi = __uint_as_float(m << 16);
+        lo = -__uint_as_float(m & 0xffff0000u);
+    } else {
+        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&m));
+        hi = v.x;
+        lo = -v.y;
+    }
+}
 
 template <int D, int BS, bool BF16>
 __global__ void __launch_bounds__(kInt4Threads)
     kv_append_int4_kernel(const uint16_t* __restrict__ x, uint32_t* __restrict__ codes,
-                          uint32_t* __restrict__ params, Int4Rows g) {
+                          uint32_t* __restrict__ params, const Int4Rows g) {
     griddep_wait();
     griddep_launch_dependents();
-    constexpr int kLPR = D / 8;
-    constexpr int kRPW = 32 / kLPR;
-    const int l = (threadIdx.x & 31) % kLPR;
+    constexpr int kLanes = D / 16;
+    constexpr int kRPW = 32 / kLanes;
+    const int l = (threadIdx.x & 31) % kLanes;
     const uint32_t warp = (blockIdx.x * kInt4Threads + threadIdx.x) >> 5;
-    const uint32_t r0 = warp * (kRPW * kInt4Unroll) + (threadIdx.x & 31) / kLPR;
+    const uint32_t r0 = warp * (kRPW * kInt4Unroll) + (threadIdx.x & 31) / kLanes;
     long long row[kInt4Unroll];
     bool ok[kInt4Unroll];
-    uint4 raw[kInt4Unroll];
+    uint32_t raw[kInt4Unroll][8];
 #pragma unroll
     for (int u = 0; u < kInt4Unroll; ++u) {
         const uint32_t r = r0 + u * kRPW;
         long long off = 0;
         row[u] = 0;
         ok[u] = r < g.rows && g.locate(r, row[u], off);
-        raw[u] = make_uint4(0, 0, 0, 0);
-        if (ok[u]) raw[u] = ld_stream_v4(reinterpret_cast<const uint4*>(x + off) + l);
+        uint4 a = make_uint4(0, 0, 0, 0), b = a;
+        if (ok[u]) {
+            a = reinterpret_cast<const uint4*>(x + off)[2 * l];
+            b = reinterpret_cast<const uint4*>(x + off)[2 * l + 1];
+        }
+        raw[u][0] = a.x, raw[u][1] = a.y, raw[u][2] = a.z, raw[u][3] = a.w;
+        raw[u][4] = b.x, raw[u][5] = b.y, raw[u][6] = b.z, raw[u][7] = b.w;
     }
 #pragma unroll
     for (int u = 0; u < kInt4Unroll; ++u) {
-        float f[8];
-        unpack8<BF16>(raw[u], f);
-        store_int4<D, BS>(f, l, row[u], ok[u], codes, params);
+        float lo, hi;
+        block_range16<BS, BF16>(raw[u], lo, hi);
+        const BlockScale b = block_scale(lo, hi);
+        uint32_t w[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float f[8];
+            unpack8<BF16>(make_uint4(raw[u][4 * h], raw[u][4 * h + 1], raw[u][4 * h + 2], raw[u][4 * h + 3]), f);
+            w[h] = int4_codes(f, b);
+        }
+        if (!ok[u]) continue;
+        uint32_t* dst = codes + row[u] * (D / 8) + word_of_lane<D>(2 * l);
+        dst[0] = w[0];
+        dst[D / 32] = w[1];  // runs 2 l and 2 l + 1 are neighbours of one 32-element group
+        if (l % (BS / 16) == 0) params[row[u] * (D / BS) + l / (BS / 16)] = b.params;
     }
 }
 
@@ -254,35 +330,45 @@ __device__ __forceinline__ uint4 int4_values(uint32_t w, uint32_t params) {
 }
 
 // y[r] = the values of the cache's row; rows that the cache does not have
-// read as zero.
+// read as zero.  A lane takes runs of 8 elements r and r + 4, whose words are
+// neighbours: 8 bytes in, twice 16 out.
 template <int D, int BS, bool BF16>
 __global__ void __launch_bounds__(kInt4Threads)
     kv_reconstruct_int4_kernel(const uint32_t* __restrict__ codes,
                                const uint32_t* __restrict__ params, uint4* __restrict__ y,
-                               Int4Rows g) {
+                               const Int4Rows g) {
     griddep_wait();
     griddep_launch_dependents();
-    constexpr int kLPR = D / 8;
-    constexpr int kRPW = 32 / kLPR;
-    const int l = (threadIdx.x & 31) % kLPR;
+    constexpr int kLanes = D / 16;
+    constexpr int kRPW = 32 / kLanes;
+    const int l = (threadIdx.x & 31) % kLanes;
+    const int run = l % 4 + 8 * (l / 4);
     const uint32_t warp = (blockIdx.x * kInt4Threads + threadIdx.x) >> 5;
-    const uint32_t r0 = warp * (kRPW * kInt4Unroll) + (threadIdx.x & 31) / kLPR;
-    uint32_t w[kInt4Unroll], p[kInt4Unroll];
+    const uint32_t r0 = warp * (kRPW * kReadUnroll) + (threadIdx.x & 31) / kLanes;
+    uint2 w[kReadUnroll], p[kReadUnroll];
 #pragma unroll
-    for (int u = 0; u < kInt4Unroll; ++u) {
+    for (int u = 0; u < kReadUnroll; ++u) {
         const uint32_t r = r0 + u * kRPW;
         long long row = 0, off = 0;
-        w[u] = p[u] = 0;
+        w[u] = p[u] = make_uint2(0, 0);
         if (r < g.rows && g.locate(r, row, off)) {
-            w[u] = codes[row * (D / 8) + word_of_lane<D>(l)];
-            p[u] = params[row * (D / BS) + l / (BS / 8)];
+            w[u] = *reinterpret_cast<const uint2*>(codes + row * (D / 8) + word_of_lane<D>(run));
+            if constexpr (BS == 32) {
+                p[u] = *reinterpret_cast<const uint2*>(params + row * (D / BS) + run / 4);
+            } else {
+                p[u].x = params[row * (D / BS) + run / (BS / 8)];
+                p[u].y = p[u].x;
+            }
         }
     }
 #pragma unroll
-    for (int u = 0; u < kInt4Unroll; ++u) {
+    for (int u = 0; u < kReadUnroll; ++u) {
         const uint32_t r = r0 + u * kRPW;
-        if (r < g.rows)
-            st_stream_v4(y + static_cast<long long>(r) * kLPR + l, int4_values<BF16>(w[u], p[u]));
+        if (r < g.rows) {
+            uint4* dst = y + static_cast<long long>(r) * (D / 8) + run;
+            st_stream_v4(dst, int4_values<BF16>(w[u].x, p[u].x));
+            st_stream_v4(dst + 4, int4_values<BF16>(w[u].y, p[u].y));
+        }
     }
 }
 
@@ -297,18 +383,20 @@ __global__ void __launch_bounds__(kInt4Threads)
 // on the axis that pair j belongs to.  K rows can go straight into the 4-bit
 // cache, and V rows with them.
 //
-// The values decide 4-bit codes, where a difference in the last bit can move
-// a code, so they do not depend on the order of a sum: the mean square is
-// summed in fp64 (squares of 16-bit inputs lose nothing that fp32 would show)
-// and its reciprocal root is the fp64 one rounded to fp32; the products and
-// sums after it are rounded one by one (no contraction).
+// Values that go to the cache decide 4-bit codes, where a difference in the
+// last bit can move a code, so there (APPEND) they do not depend on the order
+// of a sum: the mean square is summed in fp64 and its reciprocal root is the
+// fp64 one rounded to fp32; the products and sums after it are rounded one by
+// one.  Without a cache all of it is fp32 with FMAs: fp64 and the separate
+// roundings add 4 us to the 33 that 8194 tokens x 40 heads of 128 take.
 //
 // A row is D / 16 lanes; a lane holds two runs of 8 elements such that the
 // halves of a pair meet in one lane (elements 8 l .. and rot / 2 + 8 l ..), so
 // the rotation needs no other lane, and 8 elements are one word of the 4-bit
-// format.  A lane group takes one token and up to heads_per_group heads of one
-// kind, so that the table's 64 bytes a lane (against 32 of data) are read once
-// for those heads.
+// format.  A warp takes one token and goes over its q, k and v heads, 512 / D
+// side by side, so that the table's 64 bytes a lane (against 32 of data a
+// head) are read once for them.  All tokens' steps, end to end, are cut into
+// equal runs, one a resident warp.
 struct RopeArgs {
     const uint16_t *q, *k, *v;     // element (b, h, t, 0) at b * sb + h * sh + t * st
     long long q_sb, q_sh, q_st, k_sb, k_sh, k_st, v_sb, v_sh, v_st;
@@ -321,11 +409,12 @@ struct RopeArgs {
     double eps;
     long long S_cap;
     uint32_t tokens;               // B * T
-    int Hq, Hkv, T, t0, max_pos, rot, heads_per_group;
-    int q_groups, kv_groups;       // lane groups a token needs for q, and for k (and for v)
+    int Hq, Hkv, T, t0, max_pos, rot;
+    int q_steps, kv_steps;         // steps of 512 / D heads: of q, of k (and of v)
+    uint32_t warps, run, longer;   // a warp takes `run` steps, the first `longer` one more
     int s1, s2, s3;                // first pair of axes 1, 2, 3
     int axes;
-    FastDiv groups, divT;          // lane groups a token needs in all
+    FastDiv steps, divT;           // steps of a token
 };
 
 // 1 / sqrt(x) rounded to fp32 as if from its exact value: one Newton step in
@@ -334,6 +423,50 @@ __device__ __forceinline__ float rsqrt_rounded(double x) {
     if (!(x > 1e-36 && x < 1e36)) return static_cast<float>(rsqrt(x));
     const double y = rsqrtf(static_cast<float>(x));
     return static_cast<float>(fma(0.5 * y, fma(-x * y, y, 1.0), y));
+}
+
+// Reciprocal root mean square of a row of D / 16 lanes, 16 elements each.
+template <int D>
+__device__ __forceinline__ float inv_rms_exact(const float (&a)[8], const float (&b)[8], double eps) {
+    double s = 0.0, t = 0.0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const double p = a[i], q = b[i];
+        s = fma(p, p, s);
+        t = fma(q, q, t);
+    }
+    s += t;
+#pragma unroll
+    for (int off = 1; off < D / 16; off <<= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+    return rsqrt_rounded(s * (1.0 / D) + eps);
+}
+
+// The same in fp32; rows whose squares leave fp32's range take the fp64 way.
+template <int D>
+__device__ __forceinline__ float inv_rms(const float (&a)[8], const float (&b)[8], double eps) {
+    float s = 0.0f, t = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        s = fmaf(a[i], a[i], s);
+        t = fmaf(b[i], b[i], t);
+    }
+    s += t;
+#pragma unroll
+    for (int off = 1; off < D / 16; off <<= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+    if (__any_sync(0xffffffffu, !(s > 1e-30f && s < 1e38f))) return inv_rms_exact<D>(a, b, eps);
+    return __frsqrt_rn(fmaf(s, 1.0f / D, static_cast<float>(eps)));
+}
+
+// (p cos - q sin, q cos + p sin), every operation rounded by itself (EXACT) or with FMAs
+template <bool EXACT>
+__device__ __forceinline__ void rotate_pair(const float p, const float q, float2 cs, float& u, float& v) {
+    if constexpr (EXACT) {
+        u = __fsub_rn(__fmul_rn(p, cs.x), __fmul_rn(q, cs.y));
+        v = __fadd_rn(__fmul_rn(q, cs.x), __fmul_rn(p, cs.y));
+    } else {
+        u = fmaf(p, cs.x, -(q * cs.y));
+        v = fmaf(q, cs.x, p * cs.y);
+    }
 }
 
 // Minimum and maximum of lane runs over blocks of BS elements, 8 a lane:
@@ -368,190 +501,242 @@ __device__ __forceinline__ void store_int4_runs(const float (&a)[8], const float
     if constexpr (BS == D) lo[1] = lo[0], hi[1] = hi[0];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        uint32_t p;
-        const uint32_t w = int4_codes(h == 0 ? a : b, lo[h], hi[h], p);
+        const BlockScale s = block_scale(lo[h], hi[h]);
+        const uint32_t w = int4_codes(h == 0 ? a : b, s);
         if (!valid) continue;
         const int run = l + h * kLanes;
         codes[row * (D / 8) + word_of_lane<D>(run)] = w;
-        if (run % (BS / 8) == 0) params[row * (D / BS) + run / (BS / 8)] = p;
+        if (run % (BS / 8) == 0) params[row * (D / BS) + run / (BS / 8)] = s.params;
     }
 }
 
-constexpr int kRopeUnroll = 2;  // heads whose rows a lane group has in flight
+constexpr int kRopeDepth = 4;  // 1 KB a warp and step: 64 KB of an SM's 16 warps in flight
 
 template <int D, int BS, bool BF16, bool APPEND, bool INTERLEAVED>
 __global__ void __launch_bounds__(kInt4Threads, 2) qk_norm_rope_kernel(const RopeArgs a) {
     griddep_wait();
     griddep_launch_dependents();
     constexpr int kLanes = D / 16;
+    constexpr int kHeads = 32 / kLanes;  // heads a step
     const int lane = threadIdx.x & 31;
     const int l = lane % kLanes;
-    const uint32_t unit = (blockIdx.x * kInt4Threads + threadIdx.x) / kLanes;
-    uint32_t tok = a.groups.div(unit);
-    int grp = static_cast<int>(unit - tok * a.groups.d);
-    const bool live = tok < a.tokens;
-    if (!live) tok = 0, grp = 0;   // keeps the warp's shuffles whole; stores nothing
-    const uint32_t b = a.divT.div(tok);
-    const uint32_t t = tok - b * a.divT.d;
-
-    int kind = 0;  // 0: q, 1: k, 2: v
-    if (grp >= a.q_groups) {
-        grp -= a.q_groups;
-        kind = 1;
-        if (grp >= a.kv_groups) grp -= a.kv_groups, kind = 2;
-    }
-    const int h0 = grp * a.heads_per_group;
-    const int H = kind == 0 ? a.Hq : a.Hkv;
-    const int h1 = h0 + a.heads_per_group < H ? h0 + a.heads_per_group : H;
-    const uint16_t* x = kind == 0 ? a.q + b * a.q_sb + t * a.q_st
-                        : kind == 1 ? a.k + b * a.k_sb + t * a.k_st
-                                    : a.v + b * a.v_sb + t * a.v_st;
-    const long long sh = kind == 0 ? a.q_sh : kind == 1 ? a.k_sh : a.v_sh;
+    // the warp's run of all tokens' steps, end to end
+    const uint32_t unit = (blockIdx.x * kInt4Threads + threadIdx.x) >> 5;
+    if (unit >= a.warps) return;
+    const uint32_t s0 = unit * a.run + min(unit, a.longer);
+    const uint32_t s1 = s0 + a.run + (unit < a.longer ? 1u : 0u);
+    // A place in the run: a token, the kind (0: q, 1: k, 2: v) of the step's heads,
+    // the steps left of that kind, and this lane's head.
+    struct Place {
+        uint32_t tok, b, t;
+        int kind, left, h;
+    };
+    constexpr int kKinds = APPEND ? 3 : 2;
+    auto locate = [&](Place& p, uint32_t step) {
+        p.tok = a.steps.div(step);
+        p.b = a.divT.div(p.tok);
+        p.t = p.tok - p.b * a.divT.d;
+        int i = static_cast<int>(step - p.tok * a.steps.d);
+        p.kind = i < a.q_steps ? 0 : i < a.q_steps + a.kv_steps ? 1 : 2;
+        if (p.kind > 0) i -= a.q_steps;
+        if (p.kind > 1) i -= a.kv_steps;
+        p.left = (p.kind == 0 ? a.q_steps : a.kv_steps) - i;
+        p.h = i * kHeads + lane / kLanes;
+    };
+    // to the next step; true if its heads are not the next ones of the same kind
+    auto next = [&](Place& p) {
+        p.h += kHeads;
+        if (--p.left > 0) return false;
+        p.h = lane / kLanes;
+        if (++p.kind == kKinds) {
+            p.kind = 0;
+            ++p.tok;
+            p.b = a.divT.div(p.tok);
+            p.t = p.tok - p.b * a.divT.d;
+        }
+        p.left = p.kind == 0 ? a.q_steps : a.kv_steps;
+        return true;
+    };
+    Place cur;
+    locate(cur, s0);
 
     // runs (in units of 8 elements): the pairs' halves of the rotated part, and
-    // the halves of what is behind it
+    // the halves of what is behind it; of v, and interleaved, halves of the row
     const int rot_lanes = a.rot / 16;
-    const bool rotates = l < rot_lanes && kind != 2;
-    const bool natural = INTERLEAVED || a.rot == D || kind == 2;  // runs l and l + kLanes
-    const int run0 = natural || l < rot_lanes ? l : rot_lanes + l;
-    const int run1 = natural ? l + kLanes : l < rot_lanes ? rot_lanes + l : kLanes + l;
-    float2 cs[8];
-    bool turns[2] = {rotates, rotates};  // interleaved: whether run 0 and run 1 rotate
-    if (INTERLEAVED) {
-        turns[0] = kind != 2 && run0 < 2 * rot_lanes;
-        turns[1] = kind != 2 && run1 < 2 * rot_lanes;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int j = INTERLEAVED ? (i < 4 ? run0 : run1) * 4 + (i & 3) : l * 8 + i;
-        cs[i] = make_float2(1.0f, 0.0f);
-        if (turns[INTERLEAVED ? i >> 2 : 0]) {
-            const int axis = a.axes == 1 ? 0 : (j >= a.s1) + (j >= a.s2) + (j >= a.s3);
-            const int p = a.pos[static_cast<long long>(axis) * a.tokens + tok];
-            // a position outside the table leaves NaN in the row
-            cs[i] = p >= 0 && p < a.max_pos
-                        ? a.table[static_cast<long long>(p) * (a.rot / 2) + j]
-                        : make_float2(NAN, NAN);
+    const bool natural = INTERLEAVED || a.rot == D;
+    const int pair0 = natural || l < rot_lanes ? l : rot_lanes + l;
+    const int pair1 = natural ? l + kLanes : l < rot_lanes ? rot_lanes + l : kLanes + l;
+    // rows come through shared memory, kRopeDepth steps ahead; a lane reads back
+    // what it asked for itself
+    __shared__ uint4 ring[kInt4Threads / 32][kRopeDepth][2][32];
+    uint4(*mine)[2][32] = ring[threadIdx.x >> 5];
+    Place ahead = cur;
+    uint32_t asked = s0;
+    const uint16_t *src0, *src1;  // the lane's runs of head ahead.h
+    long long src_step;
+    auto aim = [&]() {
+        const Place& p = ahead;
+        const uint16_t* x = p.kind == 0 ? a.q + p.b * a.q_sb + p.t * a.q_st
+                            : p.kind == 1 ? a.k + p.b * a.k_sb + p.t * a.k_st
+                                          : a.v + p.b * a.v_sb + p.t * a.v_st;
+        const long long sh = p.kind == 0 ? a.q_sh : p.kind == 1 ? a.k_sh : a.v_sh;
+        x += p.h * sh;
+        src0 = x + 8 * (p.kind == 2 ? l : pair0);
+        src1 = x + 8 * (p.kind == 2 ? l + kLanes : pair1);
+        src_step = sh * kHeads;
+    };
+    aim();
+    auto ask = [&]() {
+        if (asked < s1) {
+            if (ahead.h < (ahead.kind == 0 ? a.Hq : a.Hkv)) {
+                uint4(*slot)[32] = mine[(asked - s0) % kRopeDepth];
+                cp_async<16>(smem_addr(&slot[0][lane]), src0);
+                cp_async<16>(smem_addr(&slot[1][lane]), src1);
+            }
+            if (++asked < s1) {
+                if (next(ahead)) {
+                    aim();
+                } else {
+                    src0 += src_step;
+                    src1 += src_step;
+                }
+            }
         }
-    }
-    const uint16_t* wsrc = kind == 0 ? a.q_w : kind == 1 ? a.k_w : nullptr;
-    float w0[8], w1[8];
-    if (wsrc) {
-        unpack8<BF16>(reinterpret_cast<const uint4*>(wsrc)[run0], w0);
-        unpack8<BF16>(reinterpret_cast<const uint4*>(wsrc)[run1], w1);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w0[i] = w1[i] = 1.0f;
-    }
+        cp_async_commit();
+    };
+#pragma unroll 1
+    for (int i = 0; i < kRopeDepth; ++i) ask();
 
-    const bool norms = __any_sync(0xffffffffu, kind != 2);   // some row of the warp is q's or k's
-    const bool caches = __any_sync(0xffffffffu, kind != 0);  // some row goes to a cache, if any does
-    for (int hb = h0; __any_sync(0xffffffffu, hb < h1); hb += kRopeUnroll) {
-        uint4 raw[kRopeUnroll][2];
+    // cos and sin of the lane's pairs: 8 of one run pair, or 4 of each run
+    const bool turn0 = INTERLEAVED ? pair0 < 2 * rot_lanes : l < rot_lanes;
+    const bool turn1 = INTERLEAVED ? pair1 < 2 * rot_lanes : turn0;
+    float2 cs[8];
+    auto load_cs = [&](uint32_t tok) {
+        auto position = [&](int axis) { return a.pos[static_cast<long long>(axis) * a.tokens + tok]; };
+        auto axis_of = [&](int j) { return a.axes == 1 ? 0 : (j >= a.s1) + (j >= a.s2) + (j >= a.s3); };
+        // `count` pairs from j on, into cs[at ...]; a position outside the table leaves NaN in the row
+        auto fetch = [&](int at, int j, auto n) {
+            constexpr int kCount = decltype(n)::value;
+            if (axis_of(j) == axis_of(j + kCount - 1)) {
+                const int p = position(axis_of(j));
+                const bool in = p >= 0 && p < a.max_pos;
+                const float4* src = reinterpret_cast<const float4*>(
+                    a.table + (in ? static_cast<long long>(p) * (a.rot / 2) + j : 0));
 #pragma unroll
-        for (int u = 0; u < kRopeUnroll; ++u) {
-            raw[u][0] = raw[u][1] = make_uint4(0, 0, 0, 0);
-            if (hb + u < h1) {
-                const uint4* src = reinterpret_cast<const uint4*>(x + (hb + u) * sh);
-                raw[u][0] = src[run0];
-                raw[u][1] = src[run1];
+                for (int i = 0; i < kCount; i += 2) {
+                    const float4 v = in ? src[i / 2] : make_float4(NAN, NAN, NAN, NAN);
+                    cs[at + i] = make_float2(v.x, v.y);
+                    cs[at + i + 1] = make_float2(v.z, v.w);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < kCount; ++i) {
+                    const int p = position(axis_of(j + i));
+                    cs[at + i] = p >= 0 && p < a.max_pos
+                                     ? a.table[static_cast<long long>(p) * (a.rot / 2) + j + i]
+                                     : make_float2(NAN, NAN);
+                }
+            }
+        };
+        if constexpr (INTERLEAVED) {
+            if (turn0) fetch(0, pair0 * 4, std::integral_constant<int, 4>{});
+            if (turn1) fetch(4, pair1 * 4, std::integral_constant<int, 4>{});
+        } else {
+            if (turn0) fetch(0, l * 8, std::integral_constant<int, 8>{});
+        }
+    };
+
+    // where the outputs of cur's token and kind are: head 0's row of q_out or k_out,
+    // or of the caches (-1: the cache does not have it)
+    uint4* out = nullptr;
+    const long long out_head = static_cast<long long>(a.T) * (D / 8);
+    long long row0 = -1;
+    auto enter = [&]() {
+        if (!APPEND || cur.kind == 0) {
+            out = reinterpret_cast<uint4*>(cur.kind == 0 ? a.q_out : a.k_out) +
+                  (static_cast<long long>(cur.b) * (cur.kind == 0 ? a.Hq : a.Hkv) * a.T + cur.t) * (D / 8);
+        } else {
+            const long long pos = (a.starts ? static_cast<long long>(a.starts[cur.b]) : a.t0) + cur.t;
+            row0 = pos >= 0 && pos < a.S_cap ? static_cast<long long>(cur.b) * a.Hkv * a.S_cap + pos : -1;
+        }
+    };
+    enter();
+
+    float w0[8], w1[8];
+    int weights = -1;              // the kind they are of
+    uint32_t cs_tok = 0xffffffffu;  // the token cs is of
+    for (uint32_t s = s0; s < s1; ++s) {
+        const int kind = cur.kind, h = cur.h;
+        const bool store = h < (kind == 0 ? a.Hq : a.Hkv);
+        cp_async_wait<kRopeDepth - 1>();
+        uint4(*slot)[32] = mine[(s - s0) % kRopeDepth];
+        float f0[8], f1[8];  // of heads that do not exist: whatever the slot held, stored nowhere
+        unpack8<BF16>(slot[0][lane], f0);
+        unpack8<BF16>(slot[1][lane], f1);
+        if (kind != 2) {
+            if (cur.tok != cs_tok) load_cs(cs_tok = cur.tok);
+            if (kind != weights) {
+                weights = kind;
+                const uint16_t* w = kind == 0 ? a.q_w : a.k_w;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) w0[j] = w1[j] = 1.0f;
+                if (w) {
+                    unpack8<BF16>(reinterpret_cast<const uint4*>(w)[pair0], w0);
+                    unpack8<BF16>(reinterpret_cast<const uint4*>(w)[pair1], w1);
+                }
+            }
+            const float inv = APPEND ? inv_rms_exact<D>(f0, f1, a.eps) : inv_rms<D>(f0, f1, a.eps);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                f0[j] = __fmul_rn(__fmul_rn(f0[j], inv), w0[j]);
+                f1[j] = __fmul_rn(__fmul_rn(f1[j], inv), w1[j]);
+            }
+            if constexpr (INTERLEAVED) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (turn0) rotate_pair<APPEND>(f0[2 * j], f0[2 * j + 1], cs[j], f0[2 * j], f0[2 * j + 1]);
+                    if (turn1) rotate_pair<APPEND>(f1[2 * j], f1[2 * j + 1], cs[4 + j], f1[2 * j], f1[2 * j + 1]);
+                }
+            } else if (turn0) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) rotate_pair<APPEND>(f0[j], f1[j], cs[j], f0[j], f1[j]);
             }
         }
+        if (!APPEND || kind == 0) {
+            if (store) {
+                uint4* dst = out + static_cast<long long>(h) * out_head;
+                dst[pair0] = make_uint4(pack2<BF16>(f0[0], f0[1]), pack2<BF16>(f0[2], f0[3]),
+                                        pack2<BF16>(f0[4], f0[5]), pack2<BF16>(f0[6], f0[7]));
+                dst[pair1] = make_uint4(pack2<BF16>(f1[0], f1[1]), pack2<BF16>(f1[2], f1[3]),
+                                        pack2<BF16>(f1[4], f1[5]), pack2<BF16>(f1[6], f1[7]));
+            }
+        } else if constexpr (APPEND) {
+            if (!natural && kind == 1) {
+                // runs into their natural order: run r is in lane `from`, first or second
+                float n0[8], n1[8];
+                const int tail = kLanes - rot_lanes;  // lanes behind the rotated part
 #pragma unroll
-        for (int u = 0; u < kRopeUnroll; ++u) {
-            const int h = hb + u;
-            if (!__any_sync(0xffffffffu, h < h1)) break;
-            float f0[8], f1[8];
-            unpack8<BF16>(raw[u][0], f0);
-            unpack8<BF16>(raw[u][1], f1);
-            if (norms) {
-                double ss = 0.0, st = 0.0;
+                for (int s = 0; s < 2; ++s) {
+                    const int r = l + s * kLanes;
+                    const bool is_second = r < 2 * rot_lanes ? r >= rot_lanes : r - 2 * rot_lanes >= tail;
+                    const int from = lane - l + (r < 2 * rot_lanes ? (is_second ? r - rot_lanes : r)
+                                                                   : r - rot_lanes - (is_second ? tail : 0));
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const double p = f0[i], q = f1[i];
-                    ss = fma(p, p, ss);
-                    st = fma(q, q, st);
-                }
-                ss += st;
-#pragma unroll
-                for (int off = 1; off < kLanes; off <<= 1)
-                    ss += __shfl_xor_sync(0xffffffffu, ss, off);
-                if (kind != 2) {
-                    const float inv = rsqrt_rounded(ss * (1.0 / D) + a.eps);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        f0[i] = __fmul_rn(__fmul_rn(f0[i], inv), w0[i]);
-                        f1[i] = __fmul_rn(__fmul_rn(f1[i], inv), w1[i]);
-                    }
-                    if constexpr (INTERLEAVED) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            float* f = i < 4 ? f0 + 2 * i : f1 + 2 * (i - 4);
-                            if (!turns[i >> 2]) continue;
-                            const float p = f[0], q = f[1];
-                            f[0] = __fsub_rn(__fmul_rn(p, cs[i].x), __fmul_rn(q, cs[i].y));
-                            f[1] = __fadd_rn(__fmul_rn(q, cs[i].x), __fmul_rn(p, cs[i].y));
-                        }
-                    } else if (rotates) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const float p = f0[i], q = f1[i];
-                            f0[i] = __fsub_rn(__fmul_rn(p, cs[i].x), __fmul_rn(q, cs[i].y));
-                            f1[i] = __fadd_rn(__fmul_rn(q, cs[i].x), __fmul_rn(p, cs[i].y));
-                        }
+                    for (int j = 0; j < 8; ++j) {
+                        const float p = __shfl_sync(0xffffffffu, f0[j], from);
+                        const float q = __shfl_sync(0xffffffffu, f1[j], from);
+                        (s == 0 ? n0 : n1)[j] = is_second ? q : p;
                     }
                 }
-            }
-            const bool store = live && h < h1;
-            if (!APPEND || kind == 0) {
-                if (store) {
-                    uint16_t* out = kind == 0 ? a.q_out : a.k_out;
-                    const long long row = (static_cast<long long>(b) * H + h) * a.T + t;
-                    uint4* dst = reinterpret_cast<uint4*>(out) + row * (D / 8);
-                    dst[run0] = make_uint4(pack2<BF16>(f0[0], f0[1]), pack2<BF16>(f0[2], f0[3]),
-                                           pack2<BF16>(f0[4], f0[5]), pack2<BF16>(f0[6], f0[7]));
-                    dst[run1] = make_uint4(pack2<BF16>(f1[0], f1[1]), pack2<BF16>(f1[2], f1[3]),
-                                           pack2<BF16>(f1[4], f1[5]), pack2<BF16>(f1[6], f1[7]));
-                }
-            }
-            if constexpr (APPEND) {
-                if (!caches) continue;
-                if (!INTERLEAVED && a.rot != D) {
-                    // runs back into their natural order: run r is in lane `from`, first or second
-                    float n0[8], n1[8];
 #pragma unroll
-                    for (int s = 0; s < 2; ++s) {
-                        const int r = l + s * kLanes;
-                        int from = r;
-                        bool is_second = r >= kLanes;
-                        if (kind != 2) {
-                            const int tail = kLanes - rot_lanes;  // lanes behind the rotated part
-                            is_second = r < 2 * rot_lanes ? r >= rot_lanes : r - 2 * rot_lanes >= tail;
-                            from = r < 2 * rot_lanes ? (is_second ? r - rot_lanes : r)
-                                                     : r - rot_lanes - (is_second ? tail : 0);
-                        } else if (is_second) {
-                            from = r - kLanes;
-                        }
-                        from += lane - l;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const float p = __shfl_sync(0xffffffffu, f0[i], from);
-                            const float q = __shfl_sync(0xffffffffu, f1[i], from);
-                            (s == 0 ? n0 : n1)[i] = is_second ? q : p;
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) f0[i] = n0[i], f1[i] = n1[i];
-                }
-                // lanes of q rows take part in the shuffles and store nothing
-                const long long pos =
-                    static_cast<long long>(a.starts ? a.starts[b] : a.t0) + static_cast<int>(t);
-                const bool ok = store && kind != 0 && pos >= 0 && pos < a.S_cap;
-                const long long row = (static_cast<long long>(b) * a.Hkv + h) * a.S_cap + pos;
-                store_int4_runs<D, BS>(f0, f1, l, row, ok, kind == 1 ? a.kc : a.vc,
-                                       kind == 1 ? a.kp : a.vp);
+                for (int j = 0; j < 8; ++j) f0[j] = n0[j], f1[j] = n1[j];
             }
+            const bool ok = store && row0 >= 0;
+            const long long row = row0 + static_cast<long long>(h) * a.S_cap;
+            store_int4_runs<D, BS>(f0, f1, l, row, ok, kind == 1 ? a.kc : a.vc, kind == 1 ? a.kp : a.vp);
         }
+        if (s + 1 < s1 && next(cur)) enter();
+        ask();  // into the slot that has been used
     }
 }
 

@@ -64,10 +64,9 @@ tqkv_status for_shape(int D, int bs, F&& f) {
     return TQKV_ERR_UNSUPPORTED;
 }
 
-// Rows a lane group handles per launch of the write and read kernels.
 template <int D>
-unsigned rows_grid(long long rows) {
-    const long long per = (kInt4Threads / (D / 8)) * static_cast<long long>(kInt4Unroll);
+unsigned rows_grid(long long rows, int unroll) {
+    const long long per = (kInt4Threads / (D / 16)) * static_cast<long long>(unroll);
     return static_cast<unsigned>((rows + per - 1) / per);
 }
 
@@ -186,7 +185,7 @@ tqkv_status tqkv_kv_append_int4(const void* x, const long long* x_strides, uint8
         auto fn = dtype == TQKV_BF16 ? kv_append_int4_kernel<d(), bs(), true>
                                      : kv_append_int4_kernel<d(), bs(), false>;
         return from_cuda(launch_kernel_dependent(
-            fn, dim3(rows_grid<d()>(g.rows)), dim3(kInt4Threads), 0, stream,
+            fn, dim3(rows_grid<d()>(g.rows, kInt4Unroll)), dim3(kInt4Threads), 0, stream,
             static_cast<const uint16_t*>(x), reinterpret_cast<uint32_t*>(cache_q),
             static_cast<uint32_t*>(cache_s), g));
     });
@@ -212,7 +211,7 @@ tqkv_status tqkv_kv_reconstruct_int4(const uint8_t* cache_q, const void* cache_s
         auto fn = dtype == TQKV_BF16 ? kv_reconstruct_int4_kernel<d(), bs(), true>
                                      : kv_reconstruct_int4_kernel<d(), bs(), false>;
         return from_cuda(launch_kernel_dependent(
-            fn, dim3(rows_grid<d()>(g.rows)), dim3(kInt4Threads), 0, stream,
+            fn, dim3(rows_grid<d()>(g.rows, kReadUnroll)), dim3(kInt4Threads), 0, stream,
             reinterpret_cast<const uint32_t*>(cache_q), static_cast<const uint32_t*>(cache_s),
             static_cast<uint4*>(y), g));
     });
@@ -290,7 +289,7 @@ static tqkv_status rope_checked(const tqkv_norm_rope_args* p, bool append, cudaS
     if (!p->q || !p->k || !p->q_out || !p->table || !p->positions) return TQKV_ERR_NULL;
     if (append ? (!p->v || !p->kq || !p->ks || !p->vq || !p->vs) : !p->k_out) return TQKV_ERR_NULL;
     if (!aligned(p->q, 16) || !aligned(p->k, 16) || !aligned(p->q_out, 16) ||
-        !aligned(p->q_weight, 16) || !aligned(p->k_weight, 16) || !aligned(p->table, 8) ||
+        !aligned(p->q_weight, 16) || !aligned(p->k_weight, 16) || !aligned(p->table, 16) ||
         !strides_ok(p->q_strides) || !strides_ok(p->k_strides))
         return TQKV_ERR_MISALIGNED;
     if (append ? (!aligned(p->v, 16) || !strides_ok(p->v_strides) || !aligned(p->kq, 16) ||
@@ -327,19 +326,20 @@ static tqkv_status rope_checked(const tqkv_norm_rope_args* p, bool append, cudaS
     a.s1 = axes > 1 ? p->sections[0] : INT_MAX;
     a.s2 = axes > 2 ? a.s1 + p->sections[1] : INT_MAX;
     a.s3 = axes > 3 ? a.s2 + p->sections[2] : INT_MAX;
-    const int kv_kinds = append ? 2 : 1;
-    const long long rows = tokens * (p->H_q + static_cast<long long>(kv_kinds) * p->H_kv);
-    const int rows_per_cta = kInt4Threads / (D / 16);
-    // one head per lane group while that does not fill the card twice over; then several
-    a.heads_per_group = rows <= 16ll * sms * rows_per_cta ? 1 : 4 * kRopeUnroll;
-    const int hpg = a.heads_per_group;
-    a.q_groups = (p->H_q + hpg - 1) / hpg;
-    a.kv_groups = (p->H_kv + hpg - 1) / hpg;
-    const long long per_token = a.q_groups + static_cast<long long>(kv_kinds) * a.kv_groups;
-    if (per_token * tokens > INT_MAX / 2) return TQKV_ERR_INVALID_SIZE;
-    a.groups = FastDiv(static_cast<uint32_t>(per_token));
+    const int heads = 512 / D;  // a warp's step
+    a.q_steps = (p->H_q + heads - 1) / heads;
+    a.kv_steps = (p->H_kv + heads - 1) / heads;
+    const int steps = a.q_steps + (append ? 2 : 1) * a.kv_steps;
+    const long long all = tokens * steps;
+    if (all > INT_MAX) return TQKV_ERR_INVALID_SIZE;
+    const int warps_per_cta = kInt4Threads / 32;
+    const long long resident = static_cast<long long>(sms) * warps_per_cta * 2;  // launch bounds
+    a.warps = static_cast<uint32_t>(all < resident ? all : resident);
+    a.run = static_cast<uint32_t>(all) / a.warps;
+    a.longer = static_cast<uint32_t>(all) - a.run * a.warps;
+    a.steps = FastDiv(static_cast<uint32_t>(steps));
     a.divT = FastDiv(static_cast<uint32_t>(p->T));
-    const unsigned grid = static_cast<unsigned>((per_token * tokens + rows_per_cta - 1) / rows_per_cta);
+    const unsigned grid = (a.warps + warps_per_cta - 1) / warps_per_cta;
     const bool bf16 = p->dtype == TQKV_BF16, inter = p->interleaved != 0;
     auto launch = [&](auto fn) {
         return from_cuda(launch_kernel_dependent(fn, dim3(grid), dim3(kInt4Threads), 0, stream, a));

@@ -133,8 +133,9 @@ def check_attention(out, q, kq, ks, vq, vs, bs, lengths):
                            np.argwhere(bad)[:3].tolist())
 
 
-def norm_rope(x, w, cos, sin, eps, interleaved):
-    """float64 x [B, H, T, D], cos and sin [B, 1, T, pairs] -> (out, bound before rounding)."""
+def norm_rope(x, w, cos, sin, eps, interleaved, exact=False):
+    """float64 x [B, H, T, D], cos and sin [B, 1, T, pairs] -> (out, bound before rounding);
+    `exact`: the root mean square is correct to fp32, as where the values go to a cache."""
     D, P = x.shape[-1], cos.shape[-1]
     y = x / np.sqrt((x * x).mean(-1, keepdims=True) + eps)
     if w is not None:
@@ -146,5 +147,7 @@ def norm_rope(x, w, cos, sin, eps, interleaved):
     out[..., ia], out[..., ib] = a * cos - b * sin, b * cos + a * sin
     mag[..., ia] = np.abs(a * cos) + np.abs(b * sin)
     mag[..., ib] = np.abs(b * cos) + np.abs(a * sin)
-    # 1/rms, times x, times w, times cos or sin, the sum: five roundings to fp32
-    return out, 5.1 * 2.0 ** -24 * mag
+    # 1/rms, times x, times w, times cos or sin, the sum: five roundings to fp32.  A sum of squares in
+    # fp32 passes at most 8 FMAs, 1 and 3 sums, of positive terms: 12 roundings, of which the root
+    # keeps half, and eps one, of which it keeps half
+    return out, (5.1 if exact else 5.1 + 6 + 0.5 + 0.5) * 2.0 ** -24 * mag

@@ -47,8 +47,8 @@ def _cos_sin(table, positions, sections):
     return cs[..., 0][:, None], cs[..., 1][:, None]
 
 
-def _check(out, x, w, cos, sin, eps, interleaved):
-    want, tol = norm_rope(f64(x), None if w is None else f64(w), cos, sin, eps, interleaved)
+def _check(out, x, w, cos, sin, eps, interleaved, exact=False):
+    want, tol = norm_rope(f64(x), None if w is None else f64(w), cos, sin, eps, interleaved, exact)
     u = HALF_STEP[out.dtype]
     err = np.abs(f64(out) - want)
     lim = tol * (1 + u) + u * np.abs(want) + TINY[out.dtype]
@@ -153,8 +153,8 @@ def test_append(B, Hq, Hkv, T, axes, interleaved, D, bs, dtype):
     ks, vs = (torch.full((B, Hkv, S_cap, D // bs, 2), 5.0, dtype=F16, device="cuda") for _ in "kv")
     qo = tqkv.qk_norm_rope_append_int4(q, k, v, pos, table, kq, ks, vq, vs, starts, bs, q_weight=qw,
                                        k_weight=kw, interleaved=interleaved, sections=sections)
-    _check(qo, q, qw, cos, sin, 1e-6, interleaved)
-    want_k, tol = norm_rope(f64(k), f64(kw), cos, sin, 1e-6, interleaved)
+    _check(qo, q, qw, cos, sin, 1e-6, interleaved, exact=True)
+    want_k, tol = norm_rope(f64(k), f64(kw), cos, sin, 1e-6, interleaved, exact=True)
     ref_c, ref_s = tqkv.kv_compress_int4(v, bs)
     for b, f in enumerate(first):
         rows = slice(f, f + T)
@@ -225,7 +225,7 @@ def test_prompt_then_tokens(D, bs, dtype, captured):
         for t, s in zip((kq, ks, vq, vs), saved):
             t.copy_(s)
     cos, sin = _cos_sin(table, torch.arange(S_cap)[None].expand(B, S_cap), None)
-    want_k, tol = norm_rope(f64(all_k), f64(kw), cos, sin, 1e-6, False)
+    want_k, tol = norm_rope(f64(all_k), f64(kw), cos, sin, 1e-6, False, exact=True)
     for i in range(steps):
         n = [p + i for p in prompt]
         q.copy_(_rand((B, Hq, 1, D), 100 + i, dtype))

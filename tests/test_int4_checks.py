@@ -89,7 +89,7 @@ def test_norm_rope_refusals():
             assert f(_args(**kw), None) == SIZE, kw
         for name in ("q", "k", "table", "positions", "q_out"):
             assert f(_args(**{name: None}), None) == NULL
-        for kw in (dict(q=P + 8), dict(k=P + 2), dict(q_out=P + 8), dict(q_weight=P + 8), dict(table=P + 4),
+        for kw in (dict(q=P + 8), dict(k=P + 2), dict(q_out=P + 8), dict(q_weight=P + 8), dict(table=P + 8),
                    dict(q_strides=(4, 8, 8)), dict(k_strides=(8, 8, 12))):
             assert f(_args(**kw), None) == MISALIGNED, kw
     plain, append = both
