@@ -26,11 +26,12 @@
 // error 2^-12 a token, like the 16-bit P of any tensor-core attention).  The
 // zero sums stay in fp32.
 //
-// V's codes enter as code - 8 (one packed fp16 subtraction, exact) beside zero
-// + 8 scale: sums of codes 0..15 would grow with the length while O does not,
-// and what the tensor core cuts off each sum, and p's rounding, would grow
-// with them.  K's zero terms are a product as well: a column of zeros times
-// the blocks' sums of q in two fp16 words.
+// V's codes enter as code - 8 for even tokens and code - 7 for odd ones (one
+// packed fp16 subtraction, exact) beside zero + 8 scale and zero + 7 scale:
+// sums of codes 0..15 would grow with the length while O does not, and what
+// the tensor core cuts off each sum, and p's rounding, would grow with them.
+// K's zero terms are a product as well: a column of zeros times the blocks'
+// sums of q in two fp16 words.
 //
 // Range.  p * scale must stay inside fp16 whatever the caches hold: the
 // operand is 2^(score - M - e + 11) * scale with M within 2^4 of the largest
@@ -116,8 +117,8 @@ struct I4Cfg {
     }
     // rings, the states of the units that began before a run, two descriptors a
     // warp, flags
-    static int smem_bytes(int warps, int stages, int rows) {
-        return warps * (ring(stages, rows) + state(rows) + 2 * static_cast<int>(sizeof(CutUnit))) + 16;
+    static constexpr int smem_bytes(int stages, int rows) {
+        return kWarps * (ring(stages, rows) + state(rows) + 2 * static_cast<int>(sizeof(CutUnit))) + 16;
     }
 };
 
@@ -129,12 +130,13 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// (code - 8) * 2^-U of the codes in the low (U = 24) or next (20) nibbles
+// The codes in the low (U = 24) or next (20) nibbles, less 8 in the low half (an
+// even token's) and 7 in the high one, times 2^-U.
 template <int U>
-__device__ __forceinline__ uint32_t minus8(uint32_t x) {
+__device__ __forceinline__ uint32_t centred(uint32_t x) {
     const uint32_t code = x & (U == 24 ? 0x000f000fu : 0x00f000f0u);
-    const __half2 eight = __half2half2(__ushort_as_half(U == 24 ? 0x0008 : 0x0080));
-    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&code), eight);
+    const uint32_t mid = U == 24 ? 0x00070008u : 0x00700080u;
+    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&code), *reinterpret_cast<const __half2*>(&mid));
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
@@ -143,6 +145,15 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
     uint32_t d;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
+}
+
+// Four 8 x 8 matrices of 16-bit values from shared memory, transposed: lane i
+// gives the address of row i % 8 of matrix i / 8.
+__device__ __forceinline__ void ldmatrix_trans(uint32_t (&r)[4], const uint8_t* p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(smem_addr(p))
+                 : "memory");
 }
 
 // N words from shared memory by one load
@@ -190,7 +201,7 @@ __device__ __forceinline__ void join(float4& v, float2& lr, float4 x, float2 xr)
 
 // The unit that a granule belongs to, moved forward.
 struct UnitWalk {
-    int b, u;     // sequence; (KV head, slice) within it
+    int b, kvh, slice;  // sequence; KV head and slice of its query heads
     int len, nt;  // its rows and granules
     int start;    // first granule of the unit
 
@@ -202,13 +213,21 @@ struct UnitWalk {
     __device__ __forceinline__ void seek(const Int4DecodeArgs& a, int g) {
         while (g >= start + nt && b < a.B) {
             start += nt;
-            if (nt > 0 && ++u < a.Hkv * a.slices) continue;
-            u = 0;
+            if (nt > 0) {
+                if (++slice < a.slices) continue;
+                slice = 0;
+                if (++kvh < a.Hkv) continue;
+            }
+            kvh = 0;
             ++b;
             load(a);
         }
     }
 };
+
+static_assert(I4Cfg<128, 32, 1>::smem_bytes(2, 8) <= 227 * 1024 &&
+                  I4Cfg<128, 32, 2>::smem_bytes(2, 16) <= 227 * 1024,
+              "two stages and the states of any group fit");
 
 template <int D, int BS, int NT>
 __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
@@ -216,7 +235,7 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
     using C = I4Cfg<D, BS, NT>;
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int nw = blockDim.x >> 5;
+    constexpr int nw = C::kWarps;
     const int g = lane >> 2, c = lane & 3;  // the mma's row and column groups
     const int rows = a.rec_rows;
     const int ring_bytes = C::ring(a.stages, rows);
@@ -261,24 +280,24 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
     ctas = ctas > gridDim.x ? gridDim.x : ctas < 1 ? 1 : ctas;
     const unsigned cta = blockIdx.x;
     if (cta >= ctas || n == 0) return;
-    const unsigned each = static_cast<unsigned>(n) / ctas, more = static_cast<unsigned>(n) - each * ctas;
+    const unsigned each = n / ctas, more = n - each * ctas;
     const int g0 = cta * each + (cta < more ? cta : more);
     const int g1 = g0 + each + (cta < more ? 1 : 0);
     auto cta_of = [&](unsigned tile) {
         const unsigned edge = more * (each + 1);
-        return tile < edge ? tile / (each + 1) : more + (tile - edge) / each;
+        return tile < edge ? tile / static_cast<unsigned>(each + 1) : more + static_cast<unsigned>(tile - edge) / each;
     };
     const int w0 = g0 + (g1 - g0) * warp / nw, w1 = g0 + (g1 - g0) * (warp + 1) / nw;
 
     UnitWalk walk;  // of the unit being worked on
     walk.start = 0;
     walk.b = 0;
-    walk.u = 0;
+    walk.kvh = walk.slice = 0;
     walk.len = walk.nt = 0;
     if (w0 < w1) {
         if (a.lengths == nullptr) {
             const unsigned each_b = per_seq * ((a.S + kGranule - 1) / kGranule);
-            walk.b = static_cast<unsigned>(w0) / each_b;
+            walk.b = static_cast<unsigned>(w0) / static_cast<unsigned>(each_b);
             walk.start = walk.b * each_b;
         } else {
             for (int base = 0; base < a.B; base += 32) {
@@ -302,8 +321,10 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
             }
         }
         walk.load(a);
-        walk.u = static_cast<unsigned>(w0 - walk.start) / static_cast<unsigned>(walk.nt);
-        walk.start += walk.u * walk.nt;
+        const unsigned u = static_cast<unsigned>(w0 - walk.start) / static_cast<unsigned>(walk.nt);
+        walk.kvh = a.slices == 1 ? u : u / static_cast<unsigned>(a.slices);
+        walk.slice = u - walk.kvh * a.slices;
+        walk.start += u * walk.nt;
     }
     if (lane < 2) cuts[2 * warp + lane].start = w0 < w1 ? -1 : -2;
     __syncwarp();
@@ -330,7 +351,7 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
             const int rows = (next - ahead.start) * kGranule;
             ahead_left = (rows < ahead.len ? rows : ahead.len) - t0;
             const long long row =
-                (static_cast<long long>(ahead.b) * a.Hkv + ahead.u / a.slices) * a.S_cap + t0;
+                (static_cast<long long>(ahead.b) * a.Hkv + ahead.kvh) * a.S_cap + t0;
             k_src = a.kq + row * C::kRow + lane * 16;
             kp_src = a.ks + (row + lane) * C::kNS;
         }
@@ -378,13 +399,12 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
     // elements of every 32 of head g; asked for ahead of the tiles
     uint4 q_raw[NT][C::kSub];
     auto load_q = [&](const UnitWalk& unit) {
-        const int kvh = unit.u / a.slices, slice = unit.u - kvh * a.slices;
-        const int left = a.group - slice * C::kQ;
+        const int left = a.group - unit.slice * C::kQ;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             const bool has = t * 8 + g < left;
             const uint4* src = reinterpret_cast<const uint4*>(
-                a.q + (static_cast<long long>(unit.b) * a.Hq + kvh * a.group + slice * C::kQ +
+                a.q + (static_cast<long long>(unit.b) * a.Hq + unit.kvh * a.group + unit.slice * C::kQ +
                        (has ? t * 8 + g : 0)) * D);
 #pragma unroll
             for (int b = 0; b < C::kSub; ++b)
@@ -395,12 +415,23 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
 #pragma unroll 1
     for (int i = 0; i < a.stages; ++i) issue();
 
+    const float middle = g & 1 ? 7.0f : 8.0f;  // what centred() takes off tokens g and g + 8
     const uint8_t* buf = ring;
     // this lane's place in a tile: row g's and row 2c's chunks
     const int k_at = g * C::kRow + (C::kSub == 4 ? (c ^ ((g >> 1) & 3)) * 16
                                                  : (((c >> 1) ^ ((g >> 2) & 1)) * 16 + (c & 1) * 8));
-    const int v_at = 2 * c * C::kRow + (C::kSub == 4 ? ((g >> 1) ^ c) * 16
-                                                     : (((g >> 2) ^ (c >> 1)) * 16 + ((g >> 1) & 1) * 8));
+    const int mr = lane & 7, mi = lane >> 3;  // row and matrix that it addresses
+    const int v_at =
+        BS == 128  ? mr * C::kRow + (mi ^ ((mr >> 1) & 3)) * 16
+        : BS == D  ? (mr + (mi >> 1) * 8) * C::kRow + ((mi & 1) ^ ((mr >> 2) & 1)) * 16
+        : C::kSub == 4 ? 2 * c * C::kRow + ((g >> 1) ^ c) * 16
+                       : 2 * c * C::kRow + ((g >> 2) ^ (c >> 1)) * 16 + ((g >> 1) & 1) * 8;
+    // first element of the four that row g of fragment pair b stands for
+    auto element = [&](int b) {
+        return BS == 128 ? 32 * (g >> 1) + 8 * b + 4 * (g & 1)
+               : BS == D ? 32 * ((g >> 1) & 1) + 8 * (2 * b + (g >> 2)) + 4 * (g & 1)
+                         : 32 * b + 4 * g;
+    };
 
     for (int mine = w0; mine < w1;) {
         // ---- one piece: the warp's granules [mine, p1) of one unit
@@ -409,9 +440,9 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
         const int p1 = unit_end < w1 ? unit_end : w1;
         const bool whole = mine == cur.start && p1 == unit_end;
         const bool began_before = mine != cur.start;
-        const int kvh = cur.u / a.slices, slice = cur.u - kvh * a.slices;
-        const int head0 = kvh * a.group + slice * C::kQ;
-        const int nq = a.group - slice * C::kQ < C::kQ ? a.group - slice * C::kQ : C::kQ;
+        const int head0 = cur.kvh * a.group + cur.slice * C::kQ;
+        const int left_heads = a.group - cur.slice * C::kQ;
+        const int nq = left_heads < C::kQ ? left_heads : C::kQ;
 
         // ---- q of the unit as the products' right operands
         uint32_t qf[NT][C::kSub][2][2], qz[NT];
@@ -429,9 +460,9 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
             }
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-            // 2^e with max |q| * 2^e in [2^10, 2^11): exact in fp16 down to
-            // 2^-24 of the largest element
-            int e = 137 - static_cast<int>(__float_as_uint(amax) >> 23);
+            // 2^e with max |q| * 2^e in [2^14, 2^15): exact in fp16, also over 16, down
+            // to 2^-24 of the largest element
+            int e = 141 - static_cast<int>(__float_as_uint(amax) >> 23);
             e = amax == 0.0f || amax > 3.0e38f ? 0 : e > 100 ? 100 : e < -100 ? -100 : e;
             const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
             float sum[C::kNS];
@@ -450,13 +481,14 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
                 qf[t][b][1][0] = pack2<false>(f[b][1] * 0.0625f, f[b][5] * 0.0625f);
                 qf[t][b][1][1] = pack2<false>(f[b][3] * 0.0625f, f[b][7] * 0.0625f);
             }
-            // block c's sum (below 2^18) * 2^-6 as a sum of two fp16, against its zero twice
+            // block c's sum (below 2^22) * 2^-24, the codes' unit, as a sum of two fp16, against
+            // its zero twice: off by 2^-25, or 2^-15 of the largest |q|
             float mine_sum = 0.0f;
 #pragma unroll
             for (int s = 0; s < C::kNS; ++s) {
                 sum[s] += __shfl_xor_sync(0xffffffffu, sum[s], 1);
                 sum[s] += __shfl_xor_sync(0xffffffffu, sum[s], 2);
-                if (c == s) mine_sum = sum[s] * 0.015625f;
+                if (c == s) mine_sum = sum[s] * 5.9604644775390625e-08f;
             }
             const float high = __half2float(__float2half_rn(mine_sum));
             qz[t] = pack2<false>(high, mine_sum - high);
@@ -467,8 +499,9 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
             sc[t][1] = __shfl_sync(0xffffffffu, down, 8 * c + 4);
         }
 
-        // M: largest score (base 2) that the weights are taken from; R = M + e - 11
-        float acc[NT][C::kSub][2][4], zsum[NT][C::kNS][2], M[NT][2], R[NT][2], l[NT][2];
+        // R = M + e - 11, M the largest score (base 2) so far, or up to 4 less; `limit`: the raw
+        // score beyond which R has to move
+        float acc[NT][C::kSub][2][4], zsum[NT][C::kNS][2], R[NT][2], limit[NT][2], l[NT][2];
         float scale_top = 0.0f;  // 2^e
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -478,7 +511,7 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
                 for (int i = 0; i < 8; ++i) acc[t][b][i >> 2][i & 3] = 0.0f;
 #pragma unroll
             for (int s = 0; s < C::kNS; ++s) zsum[t][s][0] = zsum[t][s][1] = 0.0f;
-            M[t][0] = M[t][1] = R[t][0] = R[t][1] = -INFINITY;
+            R[t][0] = R[t][1] = limit[t][0] = limit[t][1] = -INFINITY;
             l[t][0] = l[t][1] = 0.0f;
         }
 
@@ -513,8 +546,6 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) s[t][m][i] = 0.0f;
                     mma_f16(s[t][m], z0, z1, 0u, 0u, qz[t], 0u);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s[t][m][i] *= 3.814697265625e-06f;  // 2^(6 - 24)
                 }
                 float d[NT][4];
 #pragma unroll
@@ -577,8 +608,7 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
 #pragma unroll
                     for (int m = 1; m < C::kM; ++m)
                         top[t][j] = fmaxf(top[t][j], fmaxf(s[t][m][j], s[t][m][j + 2]));
-                    top[t][j] *= sc[t][j];
-                    over |= top[t][j] > M[t][j] + 4.0f;
+                    over |= top[t][j] > limit[t][j];
                 }
             if (__any_sync(0xffffffffu, over)) {
                 float bigf = fmaxf(__low2float(big), 5.9604644775390625e-08f);
@@ -586,6 +616,7 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
                 for (int off = 4; off < 32; off <<= 1)
                     bigf = fmaxf(bigf, __shfl_xor_sync(0xffffffffu, bigf, off));
                 // the power of two above, and its exponent
+                const float e_old = static_cast<float>(static_cast<int>(__float_as_uint(scale_top) >> 23) - 127);
                 scale_top = fmaxf(scale_top,
                                   __uint_as_float((__float_as_uint(bigf) + 0x00800000u) & 0x7f800000u));
                 const float e = static_cast<float>(static_cast<int>(__float_as_uint(scale_top) >> 23) - 127);
@@ -593,12 +624,13 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        float x = top[t][j];
+                        float x = top[t][j] * sc[t][j];
 #pragma unroll
                         for (int off = 4; off < 32; off <<= 1)
                             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
-                        M[t][j] = fmaxf(x, M[t][j]);
-                        const float r = M[t][j] + e - 11.0f;
+                        const float m = fmaxf(x, R[t][j] + (11.0f - e_old));
+                        const float r = m + e - 11.0f;
+                        limit[t][j] = (m + 4.0f) / sc[t][j];
                         const float f = r == R[t][j] ? 1.0f : fast_exp2(R[t][j] - r);
                         R[t][j] = r;
                         l[t][j] *= f;
@@ -620,13 +652,30 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
                 uint32_t q0[C::kNS], q1[C::kNS];  // parameters of rows g, g + 8
                 lds_words(q0, vp + m * 16 * 4 * C::kNS);
                 lds_words(q1, vp + (m * 16 + 8) * 4 * C::kNS);
-                // tokens 2c, 2c + 1, 2c + 8, 2c + 9 of the 16; this lane's 16 bits
-                // of each 32-element group
-                uint32_t x[4][C::kSub];
+                // 16 bits of tokens 2c, 2c + 1 (vlo) and 2c + 8, 2c + 9 (vhi): row g of the
+                // V fragments.  With one block a row any 16 bits will do, and a transposing
+                // load gives chunk b's; else row g's of the 32-element group b, so that a
+                // fragment has one scale
+                uint32_t vlo[C::kSub], vhi[C::kSub];
+                const uint8_t* vt = buf + C::kKV + v_at + m * 16 * C::kRow;
+                if constexpr (BS == 128) {
+                    ldmatrix_trans(vlo, vt);
+                    ldmatrix_trans(vhi, vt + 8 * C::kRow);
+                } else if constexpr (BS == D) {
+                    uint32_t r[4];
+                    ldmatrix_trans(r, vt);
+                    vlo[0] = r[0], vlo[1] = r[1], vhi[0] = r[2], vhi[1] = r[3];
+                } else {
+                    uint32_t x[4][C::kSub];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    lds_words(x[i], buf + C::kKV + v_at + (m * 16 + (i & 1) + (i >> 1) * 8) * C::kRow);
-                const uint32_t sel = (g & 1) ? 0x7632u : 0x5410u;
+                    for (int i = 0; i < 4; ++i) lds_words(x[i], vt + ((i & 1) + (i >> 1) * 8) * C::kRow);
+                    const uint32_t sel = (g & 1) ? 0x7632u : 0x5410u;
+#pragma unroll
+                    for (int b = 0; b < C::kSub; ++b) {
+                        vlo[b] = __byte_perm(x[0][b], x[1][b], sel);
+                        vhi[b] = __byte_perm(x[2][b], x[3][b], sel);
+                    }
+                }
                 float p[NT][4];
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
@@ -640,8 +689,8 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
                 for (int k = 0; k < C::kNS; ++k) {
                     float2 va = __half22float2(*reinterpret_cast<const __half2*>(&q0[k]));
                     float2 vb = __half22float2(*reinterpret_cast<const __half2*>(&q1[k]));
-                    va.y = fmaf(va.x, 8.0f, va.y);  // zero + 8 scale
-                    vb.y = fmaf(vb.x, 8.0f, vb.y);
+                    va.y = fmaf(va.x, middle, va.y);
+                    vb.y = fmaf(vb.x, middle, vb.y);
                     uint32_t bw[NT][2];
 #pragma unroll
                     for (int t = 0; t < NT; ++t) {
@@ -652,13 +701,12 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
                     }
 #pragma unroll
                     for (int b = k * BS / 32; b < (k + 1) * BS / 32; ++b) {
-                        const uint32_t lo = __byte_perm(x[0][b], x[1][b], sel);
-                        const uint32_t hi = __byte_perm(x[2][b], x[3][b], sel);
+                        const uint32_t lo = vlo[b], hi = vhi[b];
                         const uint32_t lo8 = lo >> 8, hi8 = hi >> 8;
-                        const uint32_t a0 = minus8<24>(lo), a1 = minus8<24>(lo8);
-                        const uint32_t a2 = minus8<24>(hi), a3 = minus8<24>(hi8);
-                        const uint32_t c0 = minus8<20>(lo), c1 = minus8<20>(lo8);
-                        const uint32_t c2 = minus8<20>(hi), c3 = minus8<20>(hi8);
+                        const uint32_t a0 = centred<24>(lo), a1 = centred<24>(lo8);
+                        const uint32_t a2 = centred<24>(hi), a3 = centred<24>(hi8);
+                        const uint32_t c0 = centred<20>(lo), c1 = centred<20>(lo8);
+                        const uint32_t c2 = centred<20>(hi), c3 = centred<20>(hi8);
 #pragma unroll
                         for (int t = 0; t < NT; ++t) {
                             mma_f16(acc[t][b][0], a0, a1, a2, a3, bw[t][0], bw[t][1]);
@@ -707,16 +755,16 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
 #pragma unroll
                 for (int b = 0; b < C::kSub; ++b) {
                     const float z = zs[b * 32 / BS];
-                    float4 v;  // elements 32 b + 4 g + {0, 1, 2, 3}
+                    float4 v;  // elements element(b) + {0, 1, 2, 3}
                     v.x = fmaf(acc[t][b][0][j], 16777216.0f, z) * inv;
                     v.y = fmaf(acc[t][b][1][j], 1048576.0f, z) * inv;
                     v.z = fmaf(acc[t][b][0][j + 2], 16777216.0f, z) * inv;
                     v.w = fmaf(acc[t][b][1][j + 2], 1048576.0f, z) * inv;
                     if (whole)
-                        store_out(a.o + (static_cast<long long>(cur.b) * a.Hq + head0 + r) * D + 32 * b + 4 * g,
+                        store_out(a.o + (static_cast<long long>(cur.b) * a.Hq + head0 + r) * D + element(b),
                                   v, bf16);
                     else
-                        *reinterpret_cast<float4*>(slot + r * C::kRecStride + 32 * b + 4 * g) = v;
+                        *reinterpret_cast<float4*>(slot + r * C::kRecStride + element(b)) = v;
                 }
                 if (!whole && g == 0)
                     *reinterpret_cast<float2*>(slot + r * C::kRecStride + D) = make_float2(ls, R[t][j]);
@@ -817,17 +865,18 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
     if (!flags[0] && !flags[1]) return;
     // all warps merge the one unit, or half of them each of the two.  A warp takes
     // a row, or, with fewer rows than warps, a run of its pieces; the loads of 8
-    // pieces (16 for D = 64) go out together
+    // pieces (16 for D = 64) go out together.  How the pieces are grouped does not
+    // depend on whether there is a second unit: sums keep their order.
     const int team = both ? nw >> 1 : nw;
     const int which = both ? (warp >= team ? 1 : 0) : (flags[0] ? 0 : 1);
     const int member = both && which ? warp - team : warp;
     const CutUnit unit = which == 0 ? before : behind;
     int log_split = 0;
-    while ((unit.nq << (log_split + 1)) <= team) ++log_split;
+    while ((unit.nq << (log_split + 1)) <= nw) ++log_split;
     const unsigned unit_first = which == 0 ? before_first : cta;
     const int np = static_cast<int>((which == 0 ? before_last : behind_last) - unit_first) + 1;
     const int rec_cta = 2 * state_floats;
-    float* parts = merge + (which && both ? (team > rows ? team : rows) : 0) * C::kRecStride;
+    float* parts = which && both ? reinterpret_cast<float*>(smem) : merge;  // the rings are free
     float* rec0 = a.recs + static_cast<long long>(unit_first) * rec_cta;
     // the first CTA's piece is its second record, all others' the first
     auto at = [&](int p) { return rec0 + static_cast<long long>(p) * rec_cta + (p == 0 ? state_floats : 0); };

@@ -107,19 +107,10 @@ DecodePlan4 plan_int4(int B, int Hq, int Hkv, int S, int D) {
     return p;
 }
 
-// Warps a CTA.
-int int4_warps(const DecodePlan4& p, int sms) {
-    const int most = p.nt == 1 ? kI4MaxWarps : 8;
-    const int w = kI4MaxWarps;
-    return w < most ? w : most;
-}
-
-// Counters and two records for every CTA that the card can hold or the tiles can feed.
-long long int4_grid(const DecodePlan4& p, int warps, int sms) {
-    long long grid = p.tiles / warps;
-    const long long resident = static_cast<long long>(sms) * ((p.nt == 1 ? kI4MaxWarps : 8) / warps);
-    if (grid > resident) grid = resident;
-    return grid < 1 ? 1 : grid;
+// One CTA an SM; a CTA has at least a tile for every warp.
+long long int4_grid(const DecodePlan4& p, int sms) {
+    const long long grid = p.tiles / (p.nt == 1 ? kI4MaxWarps : 8);
+    return grid > sms ? sms : grid < 1 ? 1 : grid;
 }
 
 size_t int4_workspace(const DecodePlan4& p, int D, long long grid) {
@@ -143,21 +134,16 @@ tqkv_status decode_int4_impl(Int4DecodeArgs a, const DecodePlan4& p, int bf16, v
         if (e != cudaSuccess) return from_cuda(e);
         opted[dev].store(true, std::memory_order_release);
     }
-    const int warps = int4_warps(p, sms);
-    long long grid = int4_grid(p, warps, sms);
+    const long long grid = int4_grid(p, sms);
     if (grid > 1 && (!workspace || workspace_bytes < int4_workspace(p, D, grid)))
         return TQKV_ERR_WORKSPACE;
-    // 1 KB of an SM's 228 KB of shared memory goes to each CTA besides its own
-    auto fit = [&](int stages) { return 228 * 1024 / (C::smem_bytes(warps, stages, p.rec_rows) + 1024); };
-    a.stages = fit(3) >= C::kWarps / warps ? 3 : 2;
-    if (fit(a.stages) < 1) return from_cuda(cudaErrorInvalidConfiguration);  // cannot happen
-    if (grid > static_cast<long long>(sms) * fit(a.stages)) grid = static_cast<long long>(sms) * fit(a.stages);
+    a.stages = C::smem_bytes(3, p.rec_rows) <= kSmem ? 3 : 2;
     if (!aligned(workspace, 16)) return TQKV_ERR_MISALIGNED;
     a.counters = static_cast<unsigned int*>(workspace);
     a.recs = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) +
                                       (static_cast<size_t>(grid) * 4 + 255) / 256 * 256);
-    return from_cuda(launch_kernel_dependent(fn, dim3(static_cast<unsigned>(grid)), dim3(32 * warps),
-                                             C::smem_bytes(warps, a.stages, p.rec_rows), stream, a, bf16));
+    return from_cuda(launch_kernel_dependent(fn, dim3(static_cast<unsigned>(grid)), dim3(32 * C::kWarps),
+                                             C::smem_bytes(a.stages, p.rec_rows), stream, a, bf16));
 }
 
 }  // namespace
@@ -223,7 +209,7 @@ size_t tqkv_decode_int4_workspace_bytes(int B, int H_q, int H_kv, int S, int D) 
     int dev = 0, sms = 0;
     if (current_sms(&dev, &sms) != cudaSuccess) return 0;
     const DecodePlan4 p = plan_int4(B, H_q, H_kv, S, D);
-    return int4_workspace(p, D, int4_grid(p, int4_warps(p, sms), sms));
+    return int4_workspace(p, D, int4_grid(p, sms));
 }
 
 tqkv_status tqkv_decode_int4(const void* q, const uint8_t* kq, const void* ks, const uint8_t* vq,

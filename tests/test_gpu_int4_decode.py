@@ -176,6 +176,27 @@ def test_results_repeat_and_the_workspace_is_left_zeroed():
     assert not ws.buf.any()
 
 
+@pytest.mark.parametrize("lengths,G", [([1, 5999], 4), ([3000, 2999], 1), ([2500, 700, 4000], 8),
+                                       ([5000, 3], 12)])
+def test_sums_keep_their_order(lengths, G):
+    """A block that arrives last at two cut units merges both at once, at other times one: the
+    bits are the same, call after call, alone and beside another call."""
+    B, S = len(lengths), 6000
+    sets = []
+    for i in range(2):
+        q = _rand((B, 2 * G, 128), 10 * i)
+        sets.append((q, *_cache(B, 2, S, 128, 64, 10 * i + 1), *_cache(B, 2, S, 128, 64, 10 * i + 2)))
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    want = [tqkv.decode_int4(*s, 64, lengths=n) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    for i in range(150):
+        got = [tqkv.decode_int4(*s, 64, lengths=n, stream=st if i % 2 else None)
+               for s, st in zip(sets, streams)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), i
+
+
 def test_workspace_shared_with_the_int8_decode():
     ws = Workspace()
     B, H, S, D, bs = 1, 4, 30000, 128, 64
