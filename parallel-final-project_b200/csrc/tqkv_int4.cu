@@ -240,7 +240,7 @@ tqkv_status tqkv_decode_int4(const void* q, const uint8_t* kq, const void* ks, c
     a.S = S;
     a.score_scale = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(D)));
     const DecodePlan4 p = plan_int4(B, H_q, H_kv, S, D);
-    if (p.granules > INT_MAX) return TQKV_ERR_INVALID_SIZE;
+    if (p.granules + p.units * kUnitCost > INT_MAX) return TQKV_ERR_INVALID_SIZE;
     a.slices = p.slices;
     a.rec_rows = p.rec_rows;
     const int bf16 = dtype == TQKV_BF16;
