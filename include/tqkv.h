@@ -397,7 +397,7 @@ tqkv_status tqkv_kv_reconstruct_int4(const uint8_t* cache_q, const void* cache_s
  * (device, int32 [B]; values are taken into [0, S]), or over S rows if
  * `lengths` is null; a sequence of no rows gives zeros.  Rows behind the
  * length are not read.  S <= S_cap only bounds the work split when there are
- * lengths.
+ * lengths.  S <= 2^31 - 1025, and B * H_kv * S below about 2^35.
  * The query heads of a K/V head (up to 8, or 16 in two halves) share one pass
  * over its rows.  Workspace as for tqkv_decode_int8 (zeroed once by
  * tqkv_workspace_init, left zeroed by every call, calls that share it

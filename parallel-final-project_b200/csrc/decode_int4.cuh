@@ -205,7 +205,7 @@ __device__ __forceinline__ void join(float4& v, float2& lr, float4 x, float2 xr)
 
 // Granules that a unit of `len` rows counts for.
 __device__ __forceinline__ int unit_length(int len) {
-    return len > 0 ? (len + kGranule - 1) / kGranule + kUnitCost : 0;
+    return len > 0 ? (len - 1) / kGranule + 1 + kUnitCost : 0;
 }
 
 // The unit that a place in the granules' sequence belongs to, moved forward.

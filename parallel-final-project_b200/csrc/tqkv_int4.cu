@@ -162,7 +162,7 @@ tqkv_status tqkv_kv_append_int4(const void* x, const long long* x_strides, uint8
     if (st != TQKV_OK) return st;
     if (!x || !cache_q || !cache_s) return TQKV_ERR_NULL;
     if (!aligned(x, 16) || !aligned(cache_q, 16) || !aligned(cache_s, 16) ||
-        (x_strides && !strides_ok(x_strides)))
+        !aligned(starts, 4) || (x_strides && !strides_ok(x_strides)))
         return TQKV_ERR_MISALIGNED;
     g.st = x_strides ? x_strides[2] : D;
     g.sh = x_strides ? x_strides[1] : static_cast<long long>(T) * D;
@@ -191,7 +191,7 @@ tqkv_status tqkv_kv_reconstruct_int4(const uint8_t* cache_q, const void* cache_s
     const tqkv_status st = make_rows(g, B, H, T, D, S_cap, starts, t0);
     if (st != TQKV_OK) return st;
     if (!cache_q || !cache_s || !y) return TQKV_ERR_NULL;
-    if (!aligned(cache_q, 16) || !aligned(cache_s, 16) || !aligned(y, 16))
+    if (!aligned(cache_q, 16) || !aligned(cache_s, 16) || !aligned(y, 16) || !aligned(starts, 4))
         return TQKV_ERR_MISALIGNED;
     return for_shape(D, block_size, [&](auto d, auto bs) {
         auto fn = dtype == TQKV_BF16 ? kv_reconstruct_int4_kernel<d(), bs(), true>
@@ -219,10 +219,11 @@ tqkv_status tqkv_decode_int4(const void* q, const uint8_t* kq, const void* ks, c
     if (!is_supported_int8(D, block_size) || !is_16bit(dtype)) return TQKV_ERR_UNSUPPORTED;
     if (B <= 0 || H_q <= 0 || H_kv <= 0 || H_q % H_kv != 0 || S < 0 || S_cap <= 0 || S > S_cap)
         return TQKV_ERR_INVALID_SIZE;
-    if (static_cast<long long>(B) * H_q > INT_MAX) return TQKV_ERR_INVALID_SIZE;
+    // rows are counted in 32 bits, in granules of 16
+    if (static_cast<long long>(B) * H_q > INT_MAX || S > INT_MAX - 1024) return TQKV_ERR_INVALID_SIZE;
     if (!q || !o || !kq || !ks || !vq || !vs) return TQKV_ERR_NULL;
     if (!aligned(q, 16) || !aligned(o, 16) || !aligned(kq, 16) || !aligned(vq, 16) ||
-        !aligned(ks, 16) || !aligned(vs, 16))
+        !aligned(ks, 16) || !aligned(vs, 16) || !aligned(lengths, 4))
         return TQKV_ERR_MISALIGNED;
     Int4DecodeArgs a{};
     a.q = static_cast<const uint16_t*>(q);
@@ -276,7 +277,8 @@ static tqkv_status rope_checked(const tqkv_norm_rope_args* p, bool append, cudaS
     if (append ? (!p->v || !p->kq || !p->ks || !p->vq || !p->vs) : !p->k_out) return TQKV_ERR_NULL;
     if (!aligned(p->q, 16) || !aligned(p->k, 16) || !aligned(p->q_out, 16) ||
         !aligned(p->q_weight, 16) || !aligned(p->k_weight, 16) || !aligned(p->table, 16) ||
-        !strides_ok(p->q_strides) || !strides_ok(p->k_strides))
+        !aligned(p->positions, 4) || !aligned(p->starts, 4) || !strides_ok(p->q_strides) ||
+        !strides_ok(p->k_strides))
         return TQKV_ERR_MISALIGNED;
     if (append ? (!aligned(p->v, 16) || !strides_ok(p->v_strides) || !aligned(p->kq, 16) ||
                   !aligned(p->ks, 16) || !aligned(p->vq, 16) || !aligned(p->vs, 16))

@@ -41,22 +41,24 @@ def _device(t: torch.Tensor, name: str) -> int:
     return index
 
 
-def _handle(index: int, stream) -> int:
-    """The stream to launch on, on device `index`."""
+def _elsewhere(fn, index: int, stream, *args, **kwargs):
+    """The call where it does not run on the current device and stream: enters them, so that what
+    it allocates belongs to that stream, and tells torch's allocator that the stream uses the
+    arguments.  The caller orders the streams, as for any torch operation."""
     if stream is None:
-        return _current_stream(index)
+        with torch.cuda.device(index):
+            return fn(*args, **kwargs)
     if stream.device.index != index:
         raise ValueError(f"stream is on {stream.device}, tensors are on cuda:{index}")
-    return stream.cuda_stream
-
-
-def _used(index: int, stream, *tensors) -> None:
-    """Tells torch's allocator about tensors that another stream than their own uses."""
-    if stream.cuda_stream != _current_stream(index) and \
-            not torch.cuda.is_current_stream_capturing():
-        for t in tensors:
-            if isinstance(t, torch.Tensor):
-                t.record_stream(stream)
+    with torch.cuda.stream(stream):
+        out = fn(*args, **kwargs)
+        if not torch.cuda.is_current_stream_capturing():
+            for t in (*args, *kwargs.values()):
+                if isinstance(t, Workspace):
+                    t = t.buf
+                if isinstance(t, torch.Tensor):
+                    t.record_stream(stream)
+    return out
 
 
 def _dtype(t: torch.Tensor, name: str) -> int:
@@ -121,6 +123,9 @@ def kv_compress_int4(x: torch.Tensor, block_size: int, xq: Optional[torch.Tensor
                      scales: Optional[torch.Tensor] = None, stream=None):
     """fp16 or bf16 [B, H, S, D] -> (codes uint8 [B, H, S, D // 2], scales fp16
     [B, H, S, D // block_size, 2])."""
+    index = _device(x, "x")
+    if stream is not None:
+        return _elsewhere(kv_compress_int4, index, stream, x, block_size, xq, scales)
     if x.dim() != 4:
         raise ValueError("x must be [B, H, S, D]")
     B, H, S, D = x.shape
@@ -132,7 +137,7 @@ def kv_compress_int4(x: torch.Tensor, block_size: int, xq: Optional[torch.Tensor
         scales = torch.empty((B, H, S, D // block_size, 2), dtype=_F16, device=x.device)
     if xq.dim() != 4 or xq.shape[2] != S:
         raise ValueError(f"xq {tuple(xq.shape)} does not have x's {S} rows")
-    kv_append_int4(x, xq, scales, 0, block_size, stream=stream)
+    kv_append_int4(x, xq, scales, 0, block_size)
     return xq, scales
 
 
@@ -140,9 +145,8 @@ def kv_append_int4(x: torch.Tensor, cache_q: torch.Tensor, cache_s: torch.Tensor
                    t0: Union[int, torch.Tensor], block_size: int, stream=None) -> None:
     """Quantise T tokens per head, x [B, H, T, D], into rows [t0, t0 + T) of a 4-bit cache."""
     index = _device(x, "x")
-    if _current_device() != index:
-        with torch.cuda.device(index):
-            return kv_append_int4(x, cache_q, cache_s, t0, block_size, stream)
+    if stream is not None or _current_device() != index:
+        return _elsewhere(kv_append_int4, index, stream, x, cache_q, cache_s, t0, block_size)
     dt = _dtype(x, "x")
     (Bx, Hx, T, Dx), strides = _rows(x, "x", x.dtype, index)
     (B, H, S_cap, _), D, _ = _cache(cache_q, cache_s, "cache_q", "cache_s", block_size, index)
@@ -151,11 +155,9 @@ def kv_append_int4(x: torch.Tensor, cache_q: torch.Tensor, cache_s: torch.Tensor
     starts, first = _starts(t0, B, index)
     status = load().tqkv_kv_append_int4(
         x.data_ptr(), _L3(*strides), cache_q.data_ptr(), cache_s.data_ptr(), starts, first, B, H, T,
-        D, block_size, S_cap, dt, _handle(index, stream))
+        D, block_size, S_cap, dt, _current_stream(index))
     if status:
         raise TqkvError("tqkv_kv_append_int4", status)
-    if stream is not None:
-        _used(index, stream, x, cache_q, cache_s, t0)
 
 
 def kv_reconstruct_int4(xq: torch.Tensor, scales: torch.Tensor, block_size: int,
@@ -165,9 +167,8 @@ def kv_reconstruct_int4(xq: torch.Tensor, scales: torch.Tensor, block_size: int,
     """The values of rows [t0, t0 + T) of a 4-bit cache (all of them by default): [B, H, T, D] in
     `dtype`, or in y's."""
     index = _device(xq, "xq")
-    if _current_device() != index:
-        with torch.cuda.device(index):
-            return kv_reconstruct_int4(xq, scales, block_size, y, t0, T, dtype, stream)
+    if stream is not None or _current_device() != index:
+        return _elsewhere(kv_reconstruct_int4, index, stream, xq, scales, block_size, y, t0, T, dtype)
     (B, H, S_cap, _), D, _ = _cache(xq, scales, "xq", "scales", block_size, index)
     starts, first = _starts(t0, B, index)
     if T is None:
@@ -184,11 +185,9 @@ def kv_reconstruct_int4(xq: torch.Tensor, scales: torch.Tensor, block_size: int,
         _is(y, "y", (B, H, T, D), y.dtype, index)
     status = load().tqkv_kv_reconstruct_int4(
         xq.data_ptr(), scales.data_ptr(), y.data_ptr(), starts, first, B, H, T, D, block_size,
-        S_cap, dt, _handle(index, stream))
+        S_cap, dt, _current_stream(index))
     if status:
         raise TqkvError("tqkv_kv_reconstruct_int4", status)
-    if stream is not None:
-        _used(index, stream, xq, scales, y, t0)
     return y
 
 
@@ -196,22 +195,22 @@ _default_ws: dict = {}
 _ws_bytes: dict = {}
 
 
-def _workspace(ws: Optional[Workspace], index: int, handle: int, stream, key):
-    """(address, bytes, tensor to keep) of the scratch for a decode of sizes `key`.  Without a
-    Workspace of the caller's, every stream has its own; a call that is being captured gets its own
-    buffer from the graph's memory, zeroed by the graph, so that graphs may replay side by side."""
+def _workspace(ws: Optional[Workspace], index: int, handle: int, key):
+    """(address, bytes) of the scratch for a decode of sizes `key`.  Without a Workspace of the
+    caller's, every stream has its own; a call that is being captured gets its own buffer from the
+    graph's memory, zeroed by the graph, so that graphs may replay side by side."""
     need = _ws_bytes.get((index, key))
     if need is None:
         need = int(load().tqkv_decode_int4_workspace_bytes(*key))
         if len(_ws_bytes) < 4096:
             _ws_bytes[(index, key)] = need
     if need == 0:
-        return None, 0, None
+        return None, 0
     if ws is not None:
         if ws.device.index not in (None, index):
             raise ValueError(f"workspace is on {ws.device}, tensors are on cuda:{index}")
         if ws.buf is not None and ws.buf.numel() >= need:
-            return ws.buf.data_ptr(), ws.buf.numel(), ws.buf
+            return ws.buf.data_ptr(), ws.buf.numel()
     if torch.cuda.is_current_stream_capturing():
         if ws is not None:
             raise ValueError("a Workspace cannot grow while a graph is captured: call once before "
@@ -220,13 +219,12 @@ def _workspace(ws: Optional[Workspace], index: int, handle: int, stream, key):
         # only the counters in front (4 bytes a CTA) have to be zero: no INT8 call uses this buffer
         check("tqkv_workspace_init",
               load().tqkv_workspace_init(buf.data_ptr(), min(need, 16384), handle))
-        return buf.data_ptr(), need, buf
+        return buf.data_ptr(), need
     if ws is None:
         ws = _default_ws.get((index, handle))
         if ws is None:
             ws = _default_ws[(index, handle)] = Workspace(torch.device("cuda", index))
-    ptr, size = ws.get(need, stream)
-    return ptr, size, ws.buf
+    return ws.get(need)
 
 
 def decode_int4(q: torch.Tensor, kq: torch.Tensor, ks: torch.Tensor, vq: torch.Tensor,
@@ -239,9 +237,9 @@ def decode_int4(q: torch.Tensor, kq: torch.Tensor, ks: torch.Tensor, vq: torch.T
     first lengths[b] rows (int32 [B] on the device, taken into [0, S]), or over S rows; S defaults
     to the cache's.  A sequence without rows gives zeros."""
     index = _device(q, "q")
-    if _current_device() != index:
-        with torch.cuda.device(index):
-            return decode_int4(q, kq, ks, vq, vs, block_size, S, lengths, out, workspace, stream)
+    if stream is not None or _current_device() != index:
+        return _elsewhere(decode_int4, index, stream, q, kq, ks, vq, vs, block_size, S, lengths, out,
+                          workspace)
     dt = _dtype(q, "q")
     shape, D, params = _cache(kq, ks, "kq", "ks", block_size, index)
     B, H_kv, S_cap, _ = shape
@@ -262,15 +260,13 @@ def decode_int4(q: torch.Tensor, kq: torch.Tensor, ks: torch.Tensor, vq: torch.T
         out = torch.empty_like(q)
     else:
         _is(out, "out", (B, H_q, D), q.dtype, index)
-    handle = _handle(index, stream)
-    ptr, size, buf = _workspace(workspace, index, handle, stream, (B, H_q, H_kv, S, D))
+    handle = _current_stream(index)
+    ptr, size = _workspace(workspace, index, handle, (B, H_q, H_kv, S, D))
     status = load().tqkv_decode_int4(
         q_ptr, kq.data_ptr(), ks.data_ptr(), v_ptr, vs_ptr, n, out.data_ptr(), B, H_q, H_kv, S,
         S_cap, D, block_size, dt, ptr, size, handle)
     if status:
         raise TqkvError("tqkv_decode_int4", status)
-    if stream is not None:
-        _used(index, stream, q, kq, ks, vq, vs, lengths, out, buf)
     return out
 
 
@@ -342,10 +338,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, tabl
     `sections`, the number of pairs that follow each axis.  A position outside the table gives
     NaN.  Outputs must not overlap the inputs."""
     index = _device(q, "q")
-    if _current_device() != index:
-        with torch.cuda.device(index):
-            return qk_norm_rope(q, k, positions, table, q_weight, k_weight, eps, interleaved,
-                                sections, q_out, k_out, stream)
+    if stream is not None or _current_device() != index:
+        return _elsewhere(qk_norm_rope, index, stream, q, k, positions, table, q_weight, k_weight,
+                          eps, interleaved, sections, q_out, k_out)
     a, _ = _norm_rope(index, q, k, positions, table, q_weight, k_weight, eps, interleaved, sections)
     if q_out is None:
         q_out = _new_rows(q)
@@ -356,11 +351,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, tabl
     else:
         _is(k_out, "k_out", k.shape, q.dtype, index)
     a.q_out, a.k_out = q_out.data_ptr(), k_out.data_ptr()
-    status = load().tqkv_qk_norm_rope(ctypes.byref(a), _handle(index, stream))
+    status = load().tqkv_qk_norm_rope(ctypes.byref(a), _current_stream(index))
     if status:
         raise TqkvError("tqkv_qk_norm_rope", status)
-    if stream is not None:
-        _used(index, stream, q, k, positions, table, q_weight, k_weight, q_out, k_out)
     return q_out, k_out
 
 
@@ -376,11 +369,10 @@ def qk_norm_rope_append_int4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     4-bit caches, in one launch; returns q [B, H_q, T, D].  K is quantised from fp32, without the
     rounding to its type that qk_norm_rope followed by kv_append_int4 has."""
     index = _device(q, "q")
-    if _current_device() != index:
-        with torch.cuda.device(index):
-            return qk_norm_rope_append_int4(q, k, v, positions, table, kq, ks, vq, vs, t0,
-                                            block_size, q_weight, k_weight, eps, interleaved,
-                                            sections, q_out, stream)
+    if stream is not None or _current_device() != index:
+        return _elsewhere(qk_norm_rope_append_int4, index, stream, q, k, v, positions, table, kq, ks,
+                          vq, vs, t0, block_size, q_weight, k_weight, eps, interleaved, sections,
+                          q_out)
     a, k_shape = _norm_rope(index, q, k, positions, table, q_weight, k_weight, eps, interleaved,
                             sections)
     v_shape, vst = _rows(v, "v", q.dtype, index)
@@ -402,10 +394,7 @@ def qk_norm_rope_append_int4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     else:
         _is(q_out, "q_out", q.shape, q.dtype, index)
     a.q_out = q_out.data_ptr()
-    status = load().tqkv_qk_norm_rope_append_int4(ctypes.byref(a), _handle(index, stream))
+    status = load().tqkv_qk_norm_rope_append_int4(ctypes.byref(a), _current_stream(index))
     if status:
         raise TqkvError("tqkv_qk_norm_rope_append_int4", status)
-    if stream is not None:
-        _used(index, stream, q, k, v, positions, table, kq, ks, vq, vs, t0, q_weight, k_weight,
-              q_out)
     return q_out

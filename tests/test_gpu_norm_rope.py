@@ -184,6 +184,60 @@ def test_append_drops_rows_outside_the_cache():
     assert torch.equal(kq[1, :, :1], full[0][1, :, 3:]) and torch.equal(vq[1, :, :1], full[1][1, :, 3:])
 
 
+def test_an_axis_without_pairs():
+    B, H, T, D = 1, 3, 9, 128
+    q, k = _rand((B, H, T, D), 1), _rand((B, H, T, D), 2)
+    table = tqkv.rope_table(40, D)
+    pos = _positions(B, T, 3, 40, 5)
+    for sections in ((0, 40, 24), (64, 0, 0), (3, 0, 61)):
+        for interleaved in (False, True):
+            cos, sin = _cos_sin(table, pos, sections)
+            qo, ko = tqkv.qk_norm_rope(q, k, pos, table, sections=sections, interleaved=interleaved)
+            _check(qo, q, None, cos, sin, 1e-6, interleaved)
+            _check(ko, k, None, cos, sin, 1e-6, interleaved)
+
+
+@pytest.mark.parametrize("D,rot,bs", [(128, 96, 32), (128, 32, 128), (64, 16, 32), (128, 64, 64)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_append_with_a_part_of_the_head_rotated(D, rot, bs, interleaved):
+    B, Hq, Hkv, T = 2, 3, 2, 11
+    q, k, v = (_rand((B, h, T, D), i) for i, h in enumerate((Hq, Hkv, Hkv)))
+    table, pos = tqkv.rope_table(50, rot), _positions(B, T, 1, 50, 1)
+    cos, sin = _cos_sin(table, pos, None)
+    kq, vq = (torch.empty((B, Hkv, T, D // 2), dtype=torch.uint8, device="cuda") for _ in "kv")
+    ks, vs = (torch.empty((B, Hkv, T, D // bs, 2), dtype=F16, device="cuda") for _ in "kv")
+    qo = tqkv.qk_norm_rope_append_int4(q, k, v, pos, table, kq, ks, vq, vs, 0, bs, interleaved=interleaved)
+    _check(qo, q, None, cos, sin, 1e-6, interleaved, exact=True)
+    want_k, tol = norm_rope(f64(k), None, cos, sin, 1e-6, interleaved, exact=True)
+    check_quantised(want_k, kq, ks, bs, slack=float((tol / np.abs(want_k).max(-1, keepdims=True)).max()) * 4)
+    ref_c, ref_s = tqkv.kv_compress_int4(v, bs)
+    assert torch.equal(vq, ref_c) and torch.equal(vs, ref_s)
+
+
+def test_on_another_stream():
+    """stream=: inputs made on the current stream, results read on it, ordered by events."""
+    B, H, T, D, bs = 2, 4, 300, 128, 64
+    table, pos = tqkv.rope_table(T, D), _positions(B, T, 1, T, 3)
+    q, k, v = (_rand((B, H, T, D), i) for i in range(3))
+
+    def run(**kw):
+        c, s = tqkv.kv_compress_int4(v, bs, **kw)
+        y = tqkv.kv_reconstruct_int4(c, s, bs, **kw)
+        qo, ko = tqkv.qk_norm_rope(q, k, pos, table, **kw)
+        tqkv.kv_append_int4(ko, c, s, 0, bs, **kw)
+        return y, qo, ko, c, s, tqkv.decode_int4(qo[:, :, 0].contiguous(), c, s, c, s, bs, **kw)
+    want = run()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(5):
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            q0 = run(stream=side)
+        got = q0
+        torch.cuda.current_stream().wait_stream(side)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 @pytest.mark.parametrize("captured", [False, True])
 @pytest.mark.parametrize("D,bs,dtype", [(128, 32, BF16), (64, 64, F16)])
 def test_prompt_then_tokens(D, bs, dtype, captured):
