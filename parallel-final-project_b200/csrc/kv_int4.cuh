@@ -5,7 +5,7 @@
 // Format.  A row of D elements has D / BS blocks.  Per block, all arithmetic
 // in fp32 with IEEE rounding:
 //     zero  = fp16(min x)
-//     scale = fp16((max x - min x) / 15)
+//     scale = fp16((max x - min x) * (1 / 15))          1 / 15 rounded to fp32
 //     code  = clamp(round_half_even((x - zero) / scale), 0, 15); 0 if scale = 0
 //     value = code * scale + zero
 // A block whose scale or zero is not finite (an input that is NaN, infinite or
@@ -116,15 +116,10 @@ struct BlockScale {
 // words, r + e with e = (1 - scale * r) * r: d * r + d * e has a relative
 // error below 2^-43 before its one rounding, which returns an exact
 // half-integer quotient as that half-integer.  One multiply and one FMA an
-// element instead of a division.  Division by 15 likewise: a quotient by 15
-// lies at least 1 / 30 of a step from the middle between two fp32 values, so
-// its rounding is the division's.
+// element instead of a division.
 __device__ __forceinline__ BlockScale block_scale(float lo, float hi) {
-    constexpr float k15 = 1.0f / 15.0f;
-    constexpr float k15low = static_cast<float>(1.0 / 15.0 - static_cast<double>(k15));
-    const float range = hi - lo;
     __half zero = __float2half_rn(lo);
-    __half scale = __float2half_rn(fmaf(range, k15, range * k15low));
+    __half scale = __float2half_rn((hi - lo) * (1.0f / 15.0f));
     const float s = __half2float(scale);
     BlockScale b;
     b.zero = __half2float(zero);

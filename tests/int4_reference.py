@@ -58,7 +58,7 @@ def quantise(x: np.ndarray, bs):
         lo, hi = b.min(-1), b.max(-1)
         zero = lo.astype(np.float16)
         rng = hi.astype(np.float32) - lo.astype(np.float32)
-        scale = (rng / np.float32(15)).astype(np.float16)
+        scale = (rng * (np.float32(1) / np.float32(15))).astype(np.float16)
         bad = ~(np.isfinite(zero) & np.isfinite(scale))
         zero[bad], scale[bad] = np.nan, np.nan
         s = np.where(bad | (scale == 0), 1, scale).astype(np.float64)
@@ -76,7 +76,7 @@ def check_quantised(x: np.ndarray, codes, scales, bs, slack):
     s, z = f64(scales)[..., 0], f64(scales)[..., 1]
     assert (np.abs(z - lo) <= 2.0 ** -11 * np.abs(lo) + 2.0 ** -25 + 2 * slack * big).all()
     want = (hi - lo) / 15
-    # one rounding of the difference, one of the quotient, one to fp16
+    # roundings of the difference, of 1 / 15 and of the product, and one to fp16
     assert (np.abs(s - want) <= (2.0 ** -11 + 2.0 ** -22) * want + 2.0 ** -25 + slack * big).all()
     got = unpack(codes).reshape(b.shape).astype(np.float64)
     sz = s[..., None]
