@@ -53,7 +53,7 @@
 // does not depend on which one that is.  The merging CTA zeroes the records
 // and the counter again.
 //
-// Every warp streams for itself: a ring of STAGES tiles filled by cp.async (16
+// Every warp streams for itself: a ring of two tiles filled by cp.async (16
 // bytes a lane, past L1), waited for by group, with no barrier between warps.
 // Rows behind the sequence's end are filled with zeros and are not read.
 // 16-byte chunks are exchanged within a row so that both ways the tile is read
@@ -88,7 +88,6 @@ struct Int4DecodeArgs {
     long long S_cap;
     int B, Hq, Hkv, group, slices, S;
     int rec_rows;               // query heads a record holds: min(group, 8 * NT)
-    int stages;                 // ring stages a warp has: 2 or 3
     float score_scale;          // log2(e) / sqrt(D)
 };
 
@@ -110,19 +109,22 @@ struct I4Cfg {
     static constexpr int kKV = kTile * kRow;
     static constexpr int kSc = kTile * kNS * 4;
     static constexpr int kStage = 2 * (kKV + kSc);
+    // A tile in use and one on its way.  A third stage gains 1 to 4 % where blocks of
+    // 64 and more leave the kernel waiting for memory, and costs 6 % with blocks of 32.
+    static constexpr int kStages = 2;
     static constexpr int kRecStride = D + 4;      // acc[D], l at D, R at D + 1
     static constexpr int kWarps = NT == 1 ? kI4MaxWarps : 8;  // an SM's
     // bytes of the states of `rows` query heads
     __host__ __device__ static constexpr int state(int rows) { return rows * kRecStride * 4; }
     // a warp's ring: it takes the state of the unit that goes on behind its run
     // once all its tiles are used
-    __host__ __device__ static constexpr int ring(int stages, int rows) {
-        return stages * kStage > state(rows) ? stages * kStage : state(rows);
+    __host__ __device__ static constexpr int ring(int rows) {
+        return kStages * kStage > state(rows) ? kStages * kStage : state(rows);
     }
     // rings, the states of the units that began before a run, two descriptors a
     // warp, flags
-    static constexpr int smem_bytes(int stages, int rows) {
-        return kWarps * (ring(stages, rows) + state(rows) + 2 * static_cast<int>(sizeof(CutUnit))) + 16;
+    static constexpr int smem_bytes(int rows) {
+        return kWarps * (ring(rows) + state(rows) + 2 * static_cast<int>(sizeof(CutUnit))) + 16;
     }
 };
 
@@ -237,9 +239,9 @@ struct UnitWalk {
     }
 };
 
-static_assert(I4Cfg<128, 32, 1>::smem_bytes(2, 8) <= 227 * 1024 &&
-                  I4Cfg<128, 32, 2>::smem_bytes(2, 16) <= 227 * 1024,
-              "two stages and the states of any group fit");
+static_assert(I4Cfg<128, 32, 1>::smem_bytes(8) <= 227 * 1024 &&
+                  I4Cfg<128, 32, 2>::smem_bytes(16) <= 227 * 1024,
+              "the stages and the states of any group fit");
 
 template <int D, int BS, int NT>
 __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
@@ -250,7 +252,7 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
     constexpr int nw = C::kWarps;
     const int g = lane >> 2, c = lane & 3;  // the mma's row and column groups
     const int rows = a.rec_rows;
-    const int ring_bytes = C::ring(a.stages, rows);
+    const int ring_bytes = C::ring(rows);
     const int state_floats = rows * C::kRecStride;
     uint8_t* ring = smem + warp * ring_bytes;
     float* merge = reinterpret_cast<float*>(smem + nw * ring_bytes);  // [warp] state
@@ -404,8 +406,7 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
             ahead_left -= C::kTile;
             k_src += C::kKV;
             kp_src += C::kTile * C::kNS;
-            fill += C::kStage;
-            if (fill == a.stages * C::kStage) fill = 0;
+            fill = C::kStage - fill;
         }
         cp_async_commit();  // a group for every tile, real or not, so that groups can be counted
     };
@@ -427,7 +428,7 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
     };
     if (w0 < w1) load_q(walk);
 #pragma unroll 1
-    for (int i = 0; i < a.stages; ++i) issue();
+    for (int i = 0; i < C::kStages; ++i) issue();
 
     const float middle = g & 1 ? 7.0f : 8.0f;  // what centred() takes off tokens g and g + 8
     const uint8_t* buf = ring;
@@ -541,8 +542,7 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
         const int run_rows = (p1 - cur.first()) * kGranule;
         const int piece_rows = run_rows < cur.len ? run_rows : cur.len;
         for (int left = piece_rows - (from - cur.first()) * kGranule; left > 0; left -= C::kTile) {
-            if (a.stages == 3) cp_async_wait<2>();
-            else cp_async_wait<1>();
+            cp_async_wait<C::kStages - 1>();
             __syncwarp();
             const uint8_t* kp = buf + 2 * C::kKV + g * 4 * C::kNS;
             const uint8_t* vp = kp + C::kSc;
@@ -738,8 +738,7 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
                     }
                 }
             }
-            buf += C::kStage;
-            if (buf == ring + a.stages * C::kStage) buf = ring;
+            buf = buf == ring ? ring + C::kStage : ring;
             __syncwarp();  // every lane is done with the stage: refill it
             issue();
         }

@@ -137,13 +137,12 @@ tqkv_status decode_int4_impl(Int4DecodeArgs a, const DecodePlan4& p, int bf16, v
     const long long grid = int4_grid(p, sms);
     if (grid > 1 && (!workspace || workspace_bytes < int4_workspace(p, D, grid)))
         return TQKV_ERR_WORKSPACE;
-    a.stages = C::smem_bytes(3, p.rec_rows) <= kSmem ? 3 : 2;
     if (!aligned(workspace, 16)) return TQKV_ERR_MISALIGNED;
     a.counters = static_cast<unsigned int*>(workspace);
     a.recs = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) +
                                       (static_cast<size_t>(grid) * 4 + 255) / 256 * 256);
     return from_cuda(launch_kernel_dependent(fn, dim3(static_cast<unsigned>(grid)), dim3(32 * C::kWarps),
-                                             C::smem_bytes(a.stages, p.rec_rows), stream, a, bf16));
+                                             C::smem_bytes(p.rec_rows), stream, a, bf16));
 }
 
 }  // namespace
