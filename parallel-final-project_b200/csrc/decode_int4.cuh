@@ -72,10 +72,7 @@ namespace tqkv {
 
 constexpr int kGranule = 16;     // rows by which runs are cut
 constexpr int kUnitCost = 6;     // granules that a unit counts for besides its own
-// Resident warps: 12 leave each 168 registers (16 of 128 spill, and 8 hide less
-// latency: B1 H32 S65536 at block size 128 takes 54.4 us with 12, 63.3 with 16
-// and 59.7 with 8); two tiles of accumulators (NT = 2) need 8.
-constexpr int kI4MaxWarps = 12;
+constexpr int kI4MinWarps = 8;   // fewest warps of a CTA
 
 struct Int4DecodeArgs {
     const uint16_t* q;          // [B, Hq, D]
@@ -113,7 +110,12 @@ struct I4Cfg {
     // 64 and more leave the kernel waiting for memory, and costs 6 % with blocks of 32.
     static constexpr int kStages = 2;
     static constexpr int kRecStride = D + 4;      // acc[D], l at D, R at D + 1
-    static constexpr int kWarps = NT == 1 ? kI4MaxWarps : 8;  // an SM's
+    // Warps of a CTA, one CTA an SM: 12 leave each 168 registers, 8 leave 255.  12
+    // hide more latency (B1 H32 S65536, block 128: 51.9 us, 57.2 with 8 and with 16)
+    // unless two sets of accumulators (NT = 2) or four blocks a row spill (B1 32/8
+    // heads S65536, block 32: 25.8 us with 12, 24.0 with 8).
+    static constexpr int kWarps = NT == 2 || kNS == 4 ? 8 : 12;
+    static_assert(kWarps >= kI4MinWarps, "the workspace holds a record pair for every CTA");
     // bytes of the states of `rows` query heads
     __host__ __device__ static constexpr int state(int rows) { return rows * kRecStride * 4; }
     // a warp's ring: it takes the state of the unit that goes on behind its run

@@ -108,15 +108,18 @@ DecodePlan4 plan_int4(int B, int Hq, int Hkv, int S, int D) {
 }
 
 // One CTA an SM; a CTA has at least a tile for every warp.
-long long int4_grid(const DecodePlan4& p, int sms) {
-    const long long grid = p.tiles / (p.nt == 1 ? kI4MaxWarps : 8);
+long long int4_grid(const DecodePlan4& p, int sms, int warps) {
+    const long long grid = p.tiles / warps;
     return grid > sms ? sms : grid < 1 ? 1 : grid;
 }
 
-size_t int4_workspace(const DecodePlan4& p, int D, long long grid) {
+size_t int4_counters(long long grid) { return (static_cast<size_t>(grid) * 4 + 255) / 256 * 256; }
+
+// Counters and two records for every CTA, as many as any kernel may have.
+size_t int4_workspace(const DecodePlan4& p, int D, int sms) {
+    const long long grid = int4_grid(p, sms, kI4MinWarps);
     if (grid <= 1) return 0;
-    return (static_cast<size_t>(grid) * 4 + 255) / 256 * 256 +
-           static_cast<size_t>(grid) * 2 * p.rec_rows * (D + 4) * sizeof(float);
+    return int4_counters(grid) + static_cast<size_t>(grid) * 2 * p.rec_rows * (D + 4) * sizeof(float);
 }
 
 template <int D, int BS, int NT>
@@ -134,13 +137,12 @@ tqkv_status decode_int4_impl(Int4DecodeArgs a, const DecodePlan4& p, int bf16, v
         if (e != cudaSuccess) return from_cuda(e);
         opted[dev].store(true, std::memory_order_release);
     }
-    const long long grid = int4_grid(p, sms);
-    if (grid > 1 && (!workspace || workspace_bytes < int4_workspace(p, D, grid)))
-        return TQKV_ERR_WORKSPACE;
+    const long long grid = int4_grid(p, sms, C::kWarps);
+    if (grid > 1 && (!workspace || workspace_bytes < int4_workspace(p, D, sms))) return TQKV_ERR_WORKSPACE;
     if (!aligned(workspace, 16)) return TQKV_ERR_MISALIGNED;
     a.counters = static_cast<unsigned int*>(workspace);
     a.recs = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) +
-                                      (static_cast<size_t>(grid) * 4 + 255) / 256 * 256);
+                                      int4_counters(grid));
     return from_cuda(launch_kernel_dependent(fn, dim3(static_cast<unsigned>(grid)), dim3(32 * C::kWarps),
                                              C::smem_bytes(p.rec_rows), stream, a, bf16));
 }
@@ -208,7 +210,7 @@ size_t tqkv_decode_int4_workspace_bytes(int B, int H_q, int H_kv, int S, int D) 
     int dev = 0, sms = 0;
     if (current_sms(&dev, &sms) != cudaSuccess) return 0;
     const DecodePlan4 p = plan_int4(B, H_q, H_kv, S, D);
-    return int4_workspace(p, D, int4_grid(p, sms));
+    return int4_workspace(p, D, sms);
 }
 
 tqkv_status tqkv_decode_int4(const void* q, const uint8_t* kq, const void* ks, const uint8_t* vq,
