@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from ctypes import c_float, c_int, c_size_t, c_uint32, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -38,6 +39,11 @@ class NormRopeArgs(ctypes.Structure):
         ("block_size", c_int), ("S_cap", c_int), ("dtype", c_int), ("rot_dim", c_int),
         ("max_pos", c_int), ("interleaved", c_int), ("axes", c_int), ("sections", c_int * 4),
     ]
+
+
+# The same fields in the same order, for packing them in one step: 3 pointers, 9 strides, 11
+# pointers, eps, 17 ints and the structure's tail padding.
+NORM_ROPE_PACK = struct.Struct("@3P9q11Pd17i4x")
 
 
 # C ABI: name -> (restype, argtypes)
@@ -96,8 +102,9 @@ C_ABI = {
     "tqkv_kv_reconstruct_int4": (c_int, [c_void_p] * 4 + [c_int] * 8 + [c_void_p]),
     "tqkv_decode_int4_workspace_bytes": (c_size_t, [c_int] * 5),
     "tqkv_decode_int4": (c_int, [c_void_p] * 7 + [c_int] * 8 + [c_void_p, c_size_t, c_void_p]),
-    "tqkv_qk_norm_rope": (c_int, [ctypes.POINTER(NormRopeArgs), c_void_p]),
-    "tqkv_qk_norm_rope_append_int4": (c_int, [ctypes.POINTER(NormRopeArgs), c_void_p]),
+    # a NormRopeArgs by reference, or its bytes
+    "tqkv_qk_norm_rope": (c_int, [c_void_p, c_void_p]),
+    "tqkv_qk_norm_rope_append_int4": (c_int, [c_void_p, c_void_p]),
 }
 
 # The reference's C++ launchers (include/attention.h, include/quantization.h),

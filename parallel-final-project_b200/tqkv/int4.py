@@ -18,7 +18,7 @@ from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
-from ._lib import NormRopeArgs, TqkvError, check, load
+from ._lib import NORM_ROPE_PACK, TqkvError, check, load
 from .ops import Workspace
 
 _F16 = torch.float16
@@ -282,41 +282,40 @@ def rope_table(max_pos: int, rot_dim: int, base: float = 10000.0, device=None) -
     return torch.stack((angle.cos(), angle.sin()), -1).float()
 
 
-def _norm_rope(index, q, k, positions, table, q_weight, k_weight, eps, interleaved, sections):
-    """The arguments that both forms share, and k's shape."""
-    a = NormRopeArgs()
-    a.dtype = _dtype(q, "q")
+_NO_CACHE = (0, 0, 0), 0, 0, 0, 0, 0, 0, 0, 0, 0   # v's strides, v, caches, starts, t0, block, S_cap
+
+
+def _pack(index, q, k, positions, table, q_weight, k_weight, eps, interleaved, sections, q_out, k_out,
+          append=_NO_CACHE) -> bytes:
+    """tqkv_norm_rope_args (include/tqkv.h) after the checks that both forms share."""
+    dt = _dtype(q, "q")
     dtype = q.dtype
     (B, H_q, T, D), qs = _rows(q, "q", dtype, index)
-    k_shape, kst = _rows(k, "k", dtype, index)
-    Bk, H_kv, Tk, Dk = k_shape
+    (Bk, H_kv, Tk, Dk), kst = _rows(k, "k", dtype, index)
     if Bk != B or Tk != T or Dk != D:
         raise ValueError(f"k {tuple(k.shape)} does not match q {tuple(q.shape)}")
     if table.dim() != 3:
         raise ValueError("table must be float32 [max_pos, rot_dim // 2, 2]")
     max_pos, pairs, _ = table.shape
-    a.table = _is(table, "table", (max_pos, pairs, 2), torch.float32, index)
-    if sections is None:
-        a.axes = 1
-        a.positions = _is(positions, "positions", (B, T), torch.int32, index)
-    else:
-        axes = a.axes = len(sections)
-        if not 1 <= axes <= 4 or sum(sections) != pairs or min(sections) < 0:
-            raise ValueError(f"sections {tuple(sections)}: 1 to 4 counts that sum to {pairs}")
-        a.positions = _is(positions, "positions", (axes, B, T), torch.int32, index)
-        a.sections[:axes] = sections
-    if q_weight is not None:
-        a.q_weight = _is(q_weight, "q_weight", (D,), dtype, index)
-    if k_weight is not None:
-        a.k_weight = _is(k_weight, "k_weight", (D,), dtype, index)
     if max_pos > 0x7fffffff:
         raise ValueError(f"max_pos {max_pos} does not fit 32 bits")
-    a.q, a.k = q.data_ptr(), k.data_ptr()
-    a.q_strides[:], a.k_strides[:] = qs, kst
-    a.eps = eps
-    a.B, a.H_q, a.H_kv, a.T, a.D = B, H_q, H_kv, T, D
-    a.rot_dim, a.max_pos, a.interleaved = 2 * pairs, max_pos, bool(interleaved)
-    return a, k_shape
+    t_ptr = _is(table, "table", (max_pos, pairs, 2), torch.float32, index)
+    if sections is None:
+        axes, counts = 1, (0, 0, 0, 0)
+        pos = _is(positions, "positions", (B, T), torch.int32, index)
+    else:
+        axes = len(sections)
+        if not 1 <= axes <= 4 or sum(sections) != pairs or min(sections) < 0:
+            raise ValueError(f"sections {tuple(sections)}: 1 to 4 counts that sum to {pairs}")
+        counts = (*sections, 0, 0, 0)[:4]
+        pos = _is(positions, "positions", (axes, B, T), torch.int32, index)
+    qw = 0 if q_weight is None else _is(q_weight, "q_weight", (D,), dtype, index)
+    kw = 0 if k_weight is None else _is(k_weight, "k_weight", (D,), dtype, index)
+    vst, v, kq, vq, ks, vs, starts, t0, block_size, S_cap = append
+    return NORM_ROPE_PACK.pack(
+        q.data_ptr(), k.data_ptr(), v, *qs, *kst, *vst, qw, kw, t_ptr, pos, q_out, k_out, kq, vq, ks,
+        vs, starts, eps, t0, B, H_q, H_kv, T, D, block_size, S_cap, dt, 2 * pairs, max_pos,
+        1 if interleaved else 0, axes, *counts)
 
 
 def _new_rows(t: torch.Tensor) -> torch.Tensor:
@@ -341,7 +340,6 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, tabl
     if stream is not None or _current_device() != index:
         return _elsewhere(qk_norm_rope, index, stream, q, k, positions, table, q_weight, k_weight,
                           eps, interleaved, sections, q_out, k_out)
-    a, _ = _norm_rope(index, q, k, positions, table, q_weight, k_weight, eps, interleaved, sections)
     if q_out is None:
         q_out = _new_rows(q)
     else:
@@ -350,8 +348,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, tabl
         k_out = _new_rows(k)
     else:
         _is(k_out, "k_out", k.shape, q.dtype, index)
-    a.q_out, a.k_out = q_out.data_ptr(), k_out.data_ptr()
-    status = load().tqkv_qk_norm_rope(ctypes.byref(a), _current_stream(index))
+    args = _pack(index, q, k, positions, table, q_weight, k_weight, eps, interleaved, sections,
+                 q_out.data_ptr(), k_out.data_ptr())
+    status = load().tqkv_qk_norm_rope(args, _current_stream(index))
     if status:
         raise TqkvError("tqkv_qk_norm_rope", status)
     return q_out, k_out
@@ -373,28 +372,24 @@ def qk_norm_rope_append_int4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         return _elsewhere(qk_norm_rope_append_int4, index, stream, q, k, v, positions, table, kq, ks,
                           vq, vs, t0, block_size, q_weight, k_weight, eps, interleaved, sections,
                           q_out)
-    a, k_shape = _norm_rope(index, q, k, positions, table, q_weight, k_weight, eps, interleaved,
-                            sections)
     v_shape, vst = _rows(v, "v", q.dtype, index)
-    if v_shape != k_shape:
-        raise ValueError(f"v {tuple(v_shape)} does not match k {tuple(k_shape)}")
+    if v_shape != k.shape:
+        raise ValueError(f"v {tuple(v_shape)} does not match k {tuple(k.shape)}")
     shape, D, params = _cache(kq, ks, "kq", "ks", block_size, index)
     B, H_kv, S_cap, _ = shape
-    if (B, H_kv, D) != (k_shape[0], k_shape[1], k_shape[3]):
-        raise ValueError(f"kq {tuple(kq.shape)} does not match k {tuple(k.shape)}")
-    a.vq = _is(vq, "vq", shape, _U8, index)
-    a.vs = _is(vs, "vs", params, _F16, index)
-    a.starts, a.t0 = _starts(t0, B, index)
-    a.v = v.data_ptr()
-    a.v_strides[:] = vst
-    a.kq, a.ks = kq.data_ptr(), ks.data_ptr()
-    a.block_size, a.S_cap = block_size, S_cap
+    if B != v_shape[0] or H_kv != v_shape[1] or D != v_shape[3]:
+        raise ValueError(f"kq {tuple(shape)} does not match k {tuple(k.shape)}")
+    vq_ptr = _is(vq, "vq", shape, _U8, index)
+    vs_ptr = _is(vs, "vs", params, _F16, index)
+    starts, first = _starts(t0, B, index)
     if q_out is None:
         q_out = _new_rows(q)
     else:
         _is(q_out, "q_out", q.shape, q.dtype, index)
-    a.q_out = q_out.data_ptr()
-    status = load().tqkv_qk_norm_rope_append_int4(ctypes.byref(a), _current_stream(index))
+    args = _pack(index, q, k, positions, table, q_weight, k_weight, eps, interleaved, sections,
+                 q_out.data_ptr(), 0, (vst, v.data_ptr(), kq.data_ptr(), vq_ptr, ks.data_ptr(), vs_ptr,
+                                       starts or 0, first, block_size, S_cap))
+    status = load().tqkv_qk_norm_rope_append_int4(args, _current_stream(index))
     if status:
         raise TqkvError("tqkv_qk_norm_rope_append_int4", status)
     return q_out

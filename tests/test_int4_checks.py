@@ -75,6 +75,18 @@ def _args(**kw):
     return ctypes.byref(a)
 
 
+def test_packed_arguments_are_the_structure():
+    """The front end packs tqkv_norm_rope_args in one step: every field lands where ctypes has it."""
+    n = len(_lib.NORM_ROPE_PACK.unpack(bytes(_lib.NORM_ROPE_PACK.size)))
+    assert _lib.NORM_ROPE_PACK.size == ctypes.sizeof(_lib.NormRopeArgs) and n == 41
+    a = _lib.NormRopeArgs.from_buffer_copy(_lib.NORM_ROPE_PACK.pack(*range(1, n + 1)))
+    flat = []
+    for name, _ in _lib.NormRopeArgs._fields_:
+        v = getattr(a, name)
+        flat += list(v) if hasattr(v, "__len__") else [v]
+    assert flat == list(range(1, n + 1))
+
+
 def test_norm_rope_refusals():
     lib = tqkv.load()
     both = (lib.tqkv_qk_norm_rope, lib.tqkv_qk_norm_rope_append_int4)
