@@ -181,9 +181,12 @@ struct Int4Rows {
     }
 };
 
-constexpr int kInt4Threads = 256;
-constexpr int kInt4Unroll = 2;  // rows a lane keeps in flight, 32 bytes of each
-constexpr int kReadUnroll = 4;  // and 8 bytes of each when it reads back
+// Small CTAs with little work a lane: 17.5 us for writing and reading back 131,072
+// rows of 128 in two launches, 18.4 with 256 threads and twice the rows a lane;
+// 3.5 and 4.6 us for one row of each of 512 heads.  One row a lane when reading
+// back shortens that to 3.0, but a long cache takes 136 us instead of 102.
+constexpr int kInt4Threads = 128;
+constexpr int kReadUnroll = 2;  // rows a lane has in flight when it reads back
 
 // Packed maximum of 16-bit pairs, NaN if either is.
 template <bool BF16>
@@ -245,45 +248,28 @@ __global__ void __launch_bounds__(kInt4Threads)
     griddep_wait();
     griddep_launch_dependents();
     constexpr int kLanes = D / 16;
-    constexpr int kRPW = 32 / kLanes;
-    const int l = (threadIdx.x & 31) % kLanes;
-    const uint32_t warp = (blockIdx.x * kInt4Threads + threadIdx.x) >> 5;
-    const uint32_t r0 = warp * (kRPW * kInt4Unroll) + (threadIdx.x & 31) / kLanes;
-    long long row[kInt4Unroll];
-    bool ok[kInt4Unroll];
-    uint32_t raw[kInt4Unroll][8];
-#pragma unroll
-    for (int u = 0; u < kInt4Unroll; ++u) {
-        const uint32_t r = r0 + u * kRPW;
-        long long off = 0;
-        row[u] = 0;
-        ok[u] = r < g.rows && g.locate(r, row[u], off);
-        uint4 a = make_uint4(0, 0, 0, 0), b = a;
-        if (ok[u]) {
-            a = reinterpret_cast<const uint4*>(x + off)[2 * l];
-            b = reinterpret_cast<const uint4*>(x + off)[2 * l + 1];
-        }
-        raw[u][0] = a.x, raw[u][1] = a.y, raw[u][2] = a.z, raw[u][3] = a.w;
-        raw[u][4] = b.x, raw[u][5] = b.y, raw[u][6] = b.z, raw[u][7] = b.w;
+    const int l = threadIdx.x % kLanes;
+    const uint32_t r = blockIdx.x * (kInt4Threads / kLanes) + threadIdx.x / kLanes;
+    long long row = 0, off = 0;
+    const bool ok = r < g.rows && g.locate(r, row, off);
+    uint4 a = make_uint4(0, 0, 0, 0), b = a;
+    if (ok) {
+        a = reinterpret_cast<const uint4*>(x + off)[2 * l];
+        b = reinterpret_cast<const uint4*>(x + off)[2 * l + 1];
     }
-#pragma unroll
-    for (int u = 0; u < kInt4Unroll; ++u) {
-        float lo, hi;
-        block_range16<BS, BF16>(raw[u], lo, hi);
-        const BlockScale b = block_scale(lo, hi);
-        uint32_t w[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float f[8];
-            unpack8<BF16>(make_uint4(raw[u][4 * h], raw[u][4 * h + 1], raw[u][4 * h + 2], raw[u][4 * h + 3]), f);
-            w[h] = int4_codes(f, b);
-        }
-        if (!ok[u]) continue;
-        uint32_t* dst = codes + row[u] * (D / 8) + word_of_lane<D>(2 * l);
-        dst[0] = w[0];
-        dst[D / 32] = w[1];  // runs 2 l and 2 l + 1 are neighbours of one 32-element group
-        if (l % (BS / 16) == 0) params[row[u] * (D / BS) + l / (BS / 16)] = b.params;
-    }
+    const uint32_t raw[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    float lo, hi;
+    block_range16<BS, BF16>(raw, lo, hi);
+    if (!ok) return;
+    const BlockScale scale = block_scale(lo, hi);
+    // runs 2 l and 2 l + 1 are neighbours of one 32-element group
+    uint32_t* dst = codes + row * (D / 8) + word_of_lane<D>(2 * l);
+    float f[8];
+    unpack8<BF16>(a, f);
+    dst[0] = int4_codes(f, scale);
+    unpack8<BF16>(b, f);
+    dst[D / 32] = int4_codes(f, scale);
+    if (l % (BS / 16) == 0) params[row * (D / BS) + l / (BS / 16)] = scale.params;
 }
 
 // Eight values of one packed word.  code * scale + zero is rounded once to
@@ -505,10 +491,11 @@ __device__ __forceinline__ void store_int4_runs(const float (&a)[8], const float
     }
 }
 
+constexpr int kRopeCtas = 4;   // resident on an SM
 constexpr int kRopeDepth = 4;  // 1 KB a warp and step: 64 KB of an SM's 16 warps in flight
 
 template <int D, int BS, bool BF16, bool APPEND, bool INTERLEAVED>
-__global__ void __launch_bounds__(kInt4Threads, 2) qk_norm_rope_kernel(const RopeArgs a) {
+__global__ void __launch_bounds__(kInt4Threads, kRopeCtas) qk_norm_rope_kernel(const RopeArgs a) {
     griddep_wait();
     griddep_launch_dependents();
     constexpr int kLanes = D / 16;

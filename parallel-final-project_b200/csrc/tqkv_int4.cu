@@ -172,7 +172,7 @@ tqkv_status tqkv_kv_append_int4(const void* x, const long long* x_strides, uint8
         auto fn = dtype == TQKV_BF16 ? kv_append_int4_kernel<d(), bs(), true>
                                      : kv_append_int4_kernel<d(), bs(), false>;
         return from_cuda(launch_kernel_dependent(
-            fn, dim3(rows_grid<d()>(g.rows, kInt4Unroll)), dim3(kInt4Threads), 0, stream,
+            fn, dim3(rows_grid<d()>(g.rows, 1)), dim3(kInt4Threads), 0, stream,
             static_cast<const uint16_t*>(x), reinterpret_cast<uint32_t*>(cache_q),
             static_cast<uint32_t*>(cache_s), g));
     });
@@ -322,7 +322,7 @@ static tqkv_status rope_checked(const tqkv_norm_rope_args* p, bool append, cudaS
     const long long all = tokens * steps;
     if (all > INT_MAX) return TQKV_ERR_INVALID_SIZE;
     const int warps_per_cta = kInt4Threads / 32;
-    const long long resident = static_cast<long long>(sms) * warps_per_cta * 2;  // launch bounds
+    const long long resident = static_cast<long long>(sms) * kRopeCtas * warps_per_cta;
     a.warps = static_cast<uint32_t>(all < resident ? all : resident);
     a.run = static_cast<uint32_t>(all) / a.warps;
     a.longer = static_cast<uint32_t>(all) - a.run * a.warps;
