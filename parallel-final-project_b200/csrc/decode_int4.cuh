@@ -73,6 +73,28 @@ namespace tqkv {
 constexpr int kGranule = 16;     // rows by which runs are cut
 constexpr int kUnitCost = 6;     // granules that a unit counts for besides its own
 constexpr int kI4MinWarps = 8;   // fewest warps of a CTA
+constexpr int kI4MaxWarps = 12;  // most
+constexpr int kCutTiles = 2;     // tiles a warp does in the time that joining a cut unit takes
+
+// CTAs that `n` granules of `units` units are dealt to, `most` at most: enough that each warp has
+// a tile (`per` granules a CTA), or as many as give each CTA whole units where all are as long,
+// if a warp then has less than kCutTiles tiles more.  us without the second choice and with it:
+// 16 x 8 KV heads of 300 rows (D = 128, blocks of 32) 9.9 / 6.6, 64 x 8 of 500 17.0 / 13.6 and of
+// 1 10.4 / 4.3, 8 x 12 of 1024 (D = 64) 9.6 / 7.4; 19 x 8 of 1200, where the tiles decide, 13.9 / 13.9.
+template <class I>
+__host__ __device__ inline I int4_ctas(I n, I units, I most, I per) {
+    I ctas = n / per;
+    ctas = ctas > most ? most : ctas < 1 ? 1 : ctas;
+    I whole = units;
+    if (units > most) {
+        const I each = (units + most - 1) / most;
+        whole = (units + each - 1) / each;
+    }
+    return whole >= ctas || static_cast<long long>(n) * (ctas - whole) <
+                                static_cast<long long>(kCutTiles) * per * whole * ctas
+               ? whole
+               : ctas;
+}
 
 struct Int4DecodeArgs {
     const uint16_t* q;          // [B, Hq, D]
@@ -267,6 +289,7 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
     // the first n % ctas CTAs
     const int per_seq = a.Hkv * a.slices;
     int n = 0, of_lane = 0;  // of sequence `lane`
+    int units = 0;           // sequences that hold something
     bool empty = false;
     if (a.lengths == nullptr) {
         n = a.B * unit_length(a.S);
@@ -278,9 +301,11 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
             if (b == lane) of_lane = x;
             n += x;
             empty |= len == 0;
+            units += len != 0;
         }
 #pragma unroll
         for (int off = 16; off; off >>= 1) n += __shfl_xor_sync(0xffffffffu, n, off);
+        units = __reduce_add_sync(0xffffffffu, units);
         empty = __any_sync(0xffffffffu, empty);
     }
     n *= per_seq;
@@ -291,9 +316,8 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
             for (int i = threadIdx.x; i < a.Hq * (D / 2); i += blockDim.x) o[i] = 0u;
         }
     }
-    // at least a tile for every warp of a CTA that works
-    unsigned ctas = static_cast<unsigned>(n) / (nw * C::kM);
-    ctas = ctas > gridDim.x ? gridDim.x : ctas < 1 ? 1 : ctas;
+    const unsigned ctas = a.lengths == nullptr ? gridDim.x
+                                               : int4_ctas<unsigned>(n, units * per_seq, gridDim.x, nw * C::kM);
     const unsigned cta = blockIdx.x;
     if (cta >= ctas || n == 0) return;
     const unsigned each = n / ctas, more = n - each * ctas;
@@ -303,7 +327,8 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
         const unsigned edge = more * (each + 1);
         return tile < edge ? tile / static_cast<unsigned>(each + 1) : more + static_cast<unsigned>(tile - edge) / each;
     };
-    const int w0 = g0 + (g1 - g0) * warp / nw, w1 = g0 + (g1 - g0) * (warp + 1) / nw;
+    // rounded up: warp 0 has a granule, so that a unit that began before this CTA is its first
+    const int w0 = g0 + ((g1 - g0) * warp + nw - 1) / nw, w1 = g0 + ((g1 - g0) * (warp + 1) + nw - 1) / nw;
 
     UnitWalk walk;  // of the unit being worked on
     walk.start = 0;

@@ -92,7 +92,7 @@ bool strides_ok(const long long* s) { return s[0] % 8 == 0 && s[1] % 8 == 0 && s
 struct DecodePlan4 {
     int nt, rec_rows, slices;
     long long units, granules;  // granules at most: every sequence S rows long
-    long long tiles;
+    long long counted;          // granules that they and the units count for
 };
 
 DecodePlan4 plan_int4(int B, int Hq, int Hkv, int S, int D) {
@@ -103,21 +103,22 @@ DecodePlan4 plan_int4(int B, int Hq, int Hkv, int S, int D) {
     p.slices = (group + 8 * p.nt - 1) / (8 * p.nt);
     p.units = static_cast<long long>(B) * Hkv * p.slices;
     p.granules = p.units * ((static_cast<long long>(S) + kGranule - 1) / kGranule);
-    p.tiles = p.granules / (4096 / D / kGranule);
+    p.counted = p.granules + p.units * kUnitCost;
     return p;
 }
 
-// One CTA an SM; a CTA has at least a tile for every warp.
-long long int4_grid(const DecodePlan4& p, int sms, int warps) {
-    const long long grid = p.tiles / warps;
-    return grid > sms ? sms : grid < 1 ? 1 : grid;
+// One CTA an SM at most.  Without rows (S = 0) one writes the zeros and needs no workspace.
+long long int4_grid(const DecodePlan4& p, int D, int sms, int warps) {
+    if (p.granules == 0) return 1;
+    return int4_ctas<long long>(p.counted, p.units, sms, warps * (4096 / D / kGranule));
 }
 
 size_t int4_counters(long long grid) { return (static_cast<size_t>(grid) * 4 + 255) / 256 * 256; }
 
 // Counters and two records for every CTA, as many as any kernel may have.
 size_t int4_workspace(const DecodePlan4& p, int D, int sms) {
-    const long long grid = int4_grid(p, sms, kI4MinWarps);
+    const long long few = int4_grid(p, D, sms, kI4MinWarps), many = int4_grid(p, D, sms, kI4MaxWarps);
+    const long long grid = few > many ? few : many;
     if (grid <= 1) return 0;
     return int4_counters(grid) + static_cast<size_t>(grid) * 2 * p.rec_rows * (D + 4) * sizeof(float);
 }
@@ -137,7 +138,7 @@ tqkv_status decode_int4_impl(Int4DecodeArgs a, const DecodePlan4& p, int bf16, v
         if (e != cudaSuccess) return from_cuda(e);
         opted[dev].store(true, std::memory_order_release);
     }
-    const long long grid = int4_grid(p, sms, C::kWarps);
+    const long long grid = int4_grid(p, D, sms, C::kWarps);
     if (grid > 1 && (!workspace || workspace_bytes < int4_workspace(p, D, sms))) return TQKV_ERR_WORKSPACE;
     if (!aligned(workspace, 16)) return TQKV_ERR_MISALIGNED;
     a.counters = static_cast<unsigned int*>(workspace);

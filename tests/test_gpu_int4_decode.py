@@ -67,6 +67,19 @@ def test_ragged_lengths(D, bs, G):
             assert not o[b].any()
 
 
+@pytest.mark.parametrize("D,bs", VALID)
+@pytest.mark.parametrize("B,Hkv,top", [(3, 2, 150), (2, 1, 40), (7, 3, 90), (40, 2, 60), (40, 4, 17),
+                                       (149, 1, 20), (151, 2, 140), (13, 8, 260)])
+def test_short_sequences_in_more_blocks_than_tiles(B, Hkv, top, D, bs):
+    """Blocks with fewer rows than their warps take; cuts fall at every place of a sequence."""
+    g = torch.Generator().manual_seed(B * top)
+    for lengths in ([top] * B, torch.randint(0, top + 1, (B,), generator=g).tolist()):
+        o, q, *cache = _run(B, 2 * Hkv, Hkv, top, D, bs, lengths=lengths, seed=B)
+        check_attention(o, q, *cache, bs, lengths)
+    o, q, *cache = _run(B, 2 * Hkv, Hkv, top, D, bs, seed=B)
+    check_attention(o, q, *cache, bs, [top] * B)
+
+
 def test_lengths_are_taken_into_the_range():
     lengths = [-5, 2 ** 31 - 1, -2 ** 31, 41]
     _, q, *cache = _run(4, 2, 1, 100, 128, 64)
