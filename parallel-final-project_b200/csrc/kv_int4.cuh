@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(kInt4Threads)
     constexpr int kRPW = 32 / kLanes;
     const int l = (threadIdx.x & 31) % kLanes;
     const int run = l % 4 + 8 * (l / 4);
-    const uint32_t warp = (blockIdx.x * kInt4Threads + threadIdx.x) >> 5;
+    const uint32_t warp = blockIdx.x * (kInt4Threads / 32) + threadIdx.x / 32;
     const uint32_t r0 = warp * (kRPW * kReadUnroll) + (threadIdx.x & 31) / kLanes;
     uint2 w[kReadUnroll], p[kReadUnroll];
 #pragma unroll

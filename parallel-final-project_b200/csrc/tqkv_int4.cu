@@ -259,7 +259,7 @@ static tqkv_status rope_checked(const tqkv_norm_rope_args* p, bool append, cudaS
     if ((D != 64 && D != 128) || !is_16bit(p->dtype)) return TQKV_ERR_UNSUPPORTED;
     if (append && !is_supported_int8(D, p->block_size)) return TQKV_ERR_UNSUPPORTED;
     if (rot <= 0 || rot > D || rot % 16 != 0 || axes < 1 || axes > 4) return TQKV_ERR_UNSUPPORTED;
-    int sum = 0;
+    long long sum = 0;
     for (int i = 0; i < axes; ++i) {
         if (p->sections[i] < 0) return TQKV_ERR_INVALID_SIZE;
         sum += p->sections[i];

@@ -112,11 +112,17 @@ def _cache(q: torch.Tensor, s: torch.Tensor, qn: str, sn: str, block_size: int, 
     return shape, D, params
 
 
+def _fits(n: int, name: str) -> int:
+    if not -0x80000000 <= n <= 0x7fffffff:
+        raise ValueError(f"{name} {n} does not fit 32 bits")
+    return n
+
+
 def _starts(t0: Union[int, torch.Tensor], B: int, index: int):
     """(address of the per-sequence first rows or None, first row of all)."""
     if isinstance(t0, torch.Tensor):
         return _is(t0, "t0", (B,), torch.int32, index), 0
-    return None, t0
+    return None, _fits(t0, "t0")
 
 
 def kv_compress_int4(x: torch.Tensor, block_size: int, xq: Optional[torch.Tensor] = None,
@@ -150,7 +156,7 @@ def kv_append_int4(x: torch.Tensor, cache_q: torch.Tensor, cache_s: torch.Tensor
     dt = _dtype(x, "x")
     (Bx, Hx, T, Dx), strides = _rows(x, "x", x.dtype, index)
     (B, H, S_cap, _), D, _ = _cache(cache_q, cache_s, "cache_q", "cache_s", block_size, index)
-    if B != Bx or H != Hx or D != Dx:
+    if B != Bx or H != Hx or D != Dx or T > S_cap:
         raise ValueError(f"cache_q {tuple(cache_q.shape)} does not match x {tuple(x.shape)}")
     starts, first = _starts(t0, B, index)
     status = load().tqkv_kv_append_int4(
@@ -175,6 +181,7 @@ def kv_reconstruct_int4(xq: torch.Tensor, scales: torch.Tensor, block_size: int,
         if starts is not None:
             raise ValueError("T is required with a tensor t0")
         T = S_cap - first
+    _fits(T, "T")
     if y is None:
         # scales is fp16 on the right device: the cheapest way to a tensor like it
         y = scales.new_empty((B, H, T if T > 0 else 0, D)) if dtype is _F16 else \
@@ -251,8 +258,8 @@ def decode_int4(q: torch.Tensor, kq: torch.Tensor, ks: torch.Tensor, vq: torch.T
     q_ptr = _is(q, "q", (B, H_q, D), q.dtype, index)
     if S is None:
         S = S_cap
-    elif S > 0x7fffffff:
-        raise ValueError(f"S {S} does not fit 32 bits")
+    else:
+        _fits(S, "S")
     if H_kv == 0 or H_q % H_kv:
         raise ValueError(f"H_q {H_q} is not a multiple of H_kv {H_kv}")
     n = None if lengths is None else _is(lengths, "lengths", (B,), torch.int32, index)

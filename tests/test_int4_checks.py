@@ -97,6 +97,7 @@ def test_norm_rope_refusals():
             assert f(_args(**kw), None) == UNSUPPORTED, kw
         for kw in (dict(B=0), dict(H_q=0), dict(H_kv=0), dict(T=0), dict(max_pos=0), dict(eps=-1.0),
                    dict(eps=float("nan")), dict(axes=2, sections=(32, 31)), dict(axes=2, sections=(65, -1)),
+                   dict(axes=4, sections=(2 ** 31 - 1, 2 ** 31 - 1, 2, 64)),
                    dict(B=1 << 16, T=1 << 16, S_cap=1 << 16)):
             assert f(_args(**kw), None) == SIZE, kw
         for name in ("q", "k", "table", "positions", "q_out"):
@@ -158,6 +159,27 @@ def test_python_refuses_what_does_not_fit():
     refused(int4.qk_norm_rope_append_int4, x, x, x[:, :1], pos, t, c, s, c, s, 0, 64)
     refused(int4.rope_table, 8, 24, device="cpu")
     refused(int4.rope_table, 0, 64, device="cpu")
+
+
+def test_numbers_that_a_c_int_would_cut_short(monkeypatch):
+    """ctypes takes the low 32 bits of a number: 2^32 + 1 would be row 1."""
+    monkeypatch.setattr(int4, "_device", lambda t, name: -1)
+    monkeypatch.setattr(int4, "_current_device", lambda: -1)
+    x = torch.zeros((1, 2, 8, 64), dtype=torch.float16)
+    c = torch.zeros((1, 2, 8, 32), dtype=torch.uint8)
+    s = torch.zeros((1, 2, 8, 1, 2), dtype=torch.float16)
+    q, t = torch.zeros((1, 2, 64), dtype=torch.float16), torch.zeros((8, 32, 2))
+    pos = torch.zeros((1, 8), dtype=torch.int32)
+    for far in (2 ** 32 + 1, 2 ** 31, -2 ** 32, -2 ** 31 - 1):
+        for call in (lambda: int4.kv_append_int4(x[:, :, :1], c, s, far, 64),
+                     lambda: int4.kv_reconstruct_int4(c, s, 64, t0=far, T=1),
+                     lambda: int4.kv_reconstruct_int4(c, s, 64, T=far),
+                     lambda: int4.decode_int4(q, c, s, c, s, 64, S=far),
+                     lambda: int4.qk_norm_rope_append_int4(x, x, x, pos, t, c, s, c, s, far, 64)):
+            with pytest.raises(ValueError, match="32 bits"):
+                call()
+    with pytest.raises(ValueError, match="does not match"):
+        int4.kv_append_int4(x[:, :, :1].expand(1, 2, 2 ** 32 + 1, 64), c, s, 0, 64)
 
 
 @pytest.mark.parametrize("D", [64, 128])
