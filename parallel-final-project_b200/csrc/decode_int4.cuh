@@ -23,7 +23,7 @@
 //   O       = [ sum_t (p_t scale_t) codes_t + sum_t p_t zero_t ] / sum_t p_t
 // The block scale is applied to the score in fp32; for V it is multiplied into
 // p in fp32 before p is rounded to fp16 as the product's operand (relative
-// error 2^-12 a token, like the 16-bit P of any tensor-core attention).  The
+// error 2^-11 a token, like the 16-bit P of any tensor-core attention).  The
 // zero sums stay in fp32.
 //
 // V's codes enter as code - 8 for even tokens and code - 7 for odd ones (one
