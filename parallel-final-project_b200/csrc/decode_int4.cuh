@@ -36,7 +36,17 @@
 // Range.  p * scale must stay inside fp16 whatever the caches hold: the
 // operand is 2^(score - M - e + 11) * scale with M within 2^4 of the largest
 // score so far and 2^e above the largest scale, so it is below 2^15, and
-// tokens 2^-25 of the largest keep all their bits.
+// tokens 2^-24 of the largest keep all their bits.
+//
+// Copies.  Over many tokens O is a sum of terms that cancel, and the operands'
+// rounding shows beside fp16's own: 3.2e-4 of O in the mean, where an O rounded
+// once is 2.0e-4 off (S = 131,072).  Of the 8 columns of the products a group of
+// up to 4 heads leaves half or more idle; for fp16 they hold copies of the heads
+// whose references are 1 / 2, 1 / 4 or 1 / 8 of an octave apart, so that every copy
+// rounds other numbers, and O is their mean: 2.2e-4 with 8 copies.  The stream
+// takes as long as before; the mean costs a piece 0.3 to 0.8 us (B1 H32 S65536
+// 51.9 -> 52.3 us, 512 heads of one row 4.3 -> 4.9 us).  Remainders of the weights
+// in the idle columns gave 2.0e-4, but 55.3 us.  bf16's rounding covers all of it.
 //
 // Work split.  Units are (sequence, KV head, slice of 8 * NT query heads); a
 // unit has ceil(length / 16) granules, and counts for six more, about what
@@ -107,6 +117,7 @@ struct Int4DecodeArgs {
     long long S_cap;
     int B, Hq, Hkv, group, slices, S;
     int rec_rows;               // query heads a record holds: min(group, 8 * NT)
+    int stride;                 // columns of the products from a head to its next copy: 1, 2, 4; 8 without
     float score_scale;          // log2(e) / sqrt(D)
 };
 
@@ -444,10 +455,11 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
         const int left = a.group - unit.slice * C::kQ;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            const bool has = t * 8 + g < left;
+            const int head = t * 8 + (NT == 1 ? g & (a.stride - 1) : g);
+            const bool has = head < left;
             const uint4* src = reinterpret_cast<const uint4*>(
                 a.q + (static_cast<long long>(unit.b) * a.Hq + unit.kvh * a.group + unit.slice * C::kQ +
-                       (has ? t * 8 + g : 0)) * D);
+                       (has ? head : 0)) * D);
 #pragma unroll
             for (int b = 0; b < C::kSub; ++b)
                 q_raw[t][b] = has ? src[b * 4 + c] : make_uint4(0, 0, 0, 0);
@@ -678,8 +690,10 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
 #pragma unroll
                         for (int off = 4; off < 32; off <<= 1)
                             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
-                        const float m = fmaxf(x, R[t][j] + (11.0f - e_old));
-                        const float r = m + e - 11.0f;
+                        // copy i of a head: i / copies higher
+                        const float up = NT == 1 ? 0.125f * static_cast<float>((2 * c + j) & -a.stride) : 0.0f;
+                        const float m = fmaxf(x, R[t][j] + (11.0f - e_old - up));
+                        const float r = m + (e - 11.0f + up);
                         limit[t][j] = (m + 4.0f) / sc[t][j];
                         const float f = r == R[t][j] ? 1.0f : fast_exp2(R[t][j] - r);
                         R[t][j] = r;
@@ -773,6 +787,40 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
         if (mine < w1) {
             walk.seek(a, mine);
             load_q(walk);
+        }
+
+        // ---- the mean of a head's copies, at the first one's reference
+        if (NT == 1 && a.stride < 8) {
+            const bool one = a.stride == 1;
+            const int first = (lane & ~3) | (c & ((a.stride >> 1) - (one ? 0 : 1)));
+            const float base0 = __shfl_sync(0xffffffffu, R[0][0], first);
+            const float base1 = one ? base0 : __shfl_sync(0xffffffffu, R[0][1], first);
+            const float part = 0.125f * static_cast<float>(a.stride);
+            const float f0 = R[0][0] == base0 ? part : part * fast_exp2(R[0][0] - base0);
+            const float f1 = R[0][1] == base1 ? part : part * fast_exp2(R[0][1] - base1);
+            R[0][0] = base0;
+            R[0][1] = base1;
+            auto mean = [&](float& x0, float& x1) {
+                x0 *= f0;
+                x1 *= f1;
+                if (one) x0 += x1;
+                x0 += __shfl_xor_sync(0xffffffffu, x0, 2);
+                if (!one) x1 += __shfl_xor_sync(0xffffffffu, x1, 2);
+                if (a.stride <= 2) {
+                    x0 += __shfl_xor_sync(0xffffffffu, x0, 1);
+                    if (!one) x1 += __shfl_xor_sync(0xffffffffu, x1, 1);
+                }
+            };
+            mean(l[0][0], l[0][1]);
+#pragma unroll
+            for (int k = 0; k < C::kNS; ++k) mean(zsum[0][k][0], zsum[0][k][1]);
+#pragma unroll
+            for (int b = 0; b < C::kSub; ++b)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    mean(acc[0][b][i][0], acc[0][b][i][1]);
+                    mean(acc[0][b][i][2], acc[0][b][i][3]);
+                }
         }
 
         // ---- the piece's state: to O, or to shared memory as acc[D], l, R per head

@@ -247,6 +247,8 @@ tqkv_status tqkv_decode_int4(const void* q, const uint8_t* kq, const void* ks, c
     a.slices = p.slices;
     a.rec_rows = p.rec_rows;
     const int bf16 = dtype == TQKV_BF16;
+    a.stride = 8;  // fp16: copies of the heads in the columns that a small group leaves idle
+    while (!bf16 && a.stride / 2 >= a.group) a.stride /= 2;
     return for_shape(D, block_size, [&](auto d, auto bs) {
         return p.nt == 1 ? decode_int4_impl<d(), bs(), 1>(a, p, bf16, workspace, workspace_bytes, stream)
                          : decode_int4_impl<d(), bs(), 2>(a, p, bf16, workspace, workspace_bytes, stream);

@@ -7,7 +7,7 @@ import torch
 import tqkv
 from tqkv import Workspace
 
-from int4_reference import VALID, check_attention
+from int4_reference import VALID, check_attention, f64, spread, unpack, values
 
 pytestmark = pytest.mark.gpu
 
@@ -153,6 +153,34 @@ def test_one_token_far_above_many_small_ones():
     vq, vs = tqkv.kv_compress_int4(v, bs)
     o = tqkv.decode_int4(q, kq, ks, vq, vs, bs)
     check_attention(o, q, kq, ks, vq, vs, bs, [S])
+
+
+@pytest.mark.parametrize("G,copies", [(1, 8), (2, 4), (3, 2), (4, 2)])
+def test_small_groups_average_the_rounding_of_their_weights(G, copies):
+    """fp16 over many tokens.  The error's root mean square is that of O's own rounding, known
+    exactly, and of the weights': a rounding of p * scale is uniform in half a step of at most 2^-11,
+    so 2^-11 / sqrt(3) of it at most, independent between tokens and between the copies whose mean is
+    taken.  Terms in fp32 are 2^-10 of that.  4096 elements' root mean square has a deviation of
+    1 / sqrt(8192); G * 4096 of them are here: four deviations are 4.5 %."""
+    S, D, bs, H = 12000, 128, 128, 32
+    o, q, kq, ks, vq, vs = _run(1, G * H, H, S, D, bs, seed=G)
+    kq, ks, vq, vs = (t.cpu().numpy() for t in (kq, ks, vq, vs))
+    got, qd = f64(o)[0], f64(q)[0]
+    own, weights, total = 0.0, 0.0, 0.0
+    middle = np.where(np.arange(S) % 2, 7.0, 8.0)[:, None]
+    for h in range(H):
+        s, z = spread(vs[0, h].astype(np.float64), bs)
+        c = unpack(vq[0, h]) - middle
+        k = values(kq[0, h], ks[0, h].astype(np.float64), bs)
+        for i in range(h * G, h * G + G):
+            t = k @ qd[i] / np.sqrt(D)
+            p = np.exp(t - t.max())
+            p /= p.sum()
+            want = p @ (c * s + (z + middle * s))
+            total += ((got[i] - want) ** 2).sum()
+            own += ((want.astype(np.float16) - want) ** 2).sum()
+            weights += (p ** 2 @ (c * s) ** 2).sum() * (2.0 ** -11) ** 2 / 3
+    assert total <= 1.045 ** 2 * (own + weights / copies), (total, own, weights)
 
 
 def test_bf16_queries_beyond_fp16():
