@@ -402,6 +402,8 @@ tqkv_status tqkv_kv_reconstruct_int4(const uint8_t* cache_q, const void* cache_s
  * over its rows.  Workspace as for tqkv_decode_int8 (zeroed once by
  * tqkv_workspace_init, left zeroed by every call, calls that share it
  * ordered), of tqkv_decode_int4_workspace_bytes; one workspace may serve both.
+ * Its size grows with B, S, and H_kv at one H_q / H_kv: one for the largest
+ * sizes serves all smaller ones.
  * Results do not depend on scheduling.  Programmatic dependent launches, as
  * all launches of the 4-bit cache. */
 size_t tqkv_decode_int4_workspace_bytes(int B, int H_q, int H_kv, int S, int D);

@@ -83,7 +83,6 @@ namespace tqkv {
 constexpr int kGranule = 16;     // rows by which runs are cut
 constexpr int kUnitCost = 6;     // granules that a unit counts for besides its own
 constexpr int kI4MinWarps = 8;   // fewest warps of a CTA
-constexpr int kI4MaxWarps = 12;  // most
 constexpr int kCutTiles = 2;     // tiles a warp does in the time that joining a cut unit takes
 
 // CTAs that `n` granules of `units` units are dealt to, `most` at most: enough that each warp has

@@ -115,10 +115,13 @@ long long int4_grid(const DecodePlan4& p, int D, int sms, int warps) {
 
 size_t int4_counters(long long grid) { return (static_cast<size_t>(grid) * 4 + 255) / 256 * 256; }
 
-// Counters and two records for every CTA, as many as any kernel may have.
+// Counters and two records for every CTA.  For as many CTAs as any kernel may have with these or
+// smaller sizes: the size grows with B, H_kv and S, so that a workspace for the largest batch
+// serves every smaller one (int4_ctas alone does not: 149 units may take 75 CTAs, 148 take 148).
 size_t int4_workspace(const DecodePlan4& p, int D, int sms) {
-    const long long few = int4_grid(p, D, sms, kI4MinWarps), many = int4_grid(p, D, sms, kI4MaxWarps);
-    const long long grid = few > many ? few : many;
+    const long long tiles = p.counted / (kI4MinWarps * (4096 / D / kGranule));
+    const long long most = tiles > p.units ? tiles : p.units;
+    const long long grid = p.granules == 0 ? 1 : most > sms ? sms : most;
     if (grid <= 1) return 0;
     return int4_counters(grid) + static_cast<size_t>(grid) * 2 * p.rec_rows * (D + 4) * sizeof(float);
 }

@@ -250,6 +250,31 @@ def test_workspace_shared_with_the_int8_decode():
         assert torch.equal(o4, tqkv.decode_int4(q, *c4, bs, workspace=ws))
 
 
+@pytest.mark.parametrize("G", [1, 4, 12])
+def test_a_workspace_for_the_largest_batch_serves_smaller_ones(G):
+    """Its size grows with the sizes, and the kernels take it at every batch below."""
+    need = tqkv.load().tqkv_decode_int4_workspace_bytes
+    for D in (64, 128):
+        for sizes in ([(B, H, S) for S in (1, 40, 700, 5000) for H in (1, 3) for B in range(1, 320)],
+                      [(B, 1, S) for B in (1, 149, 160) for S in range(1, 4000, 13)],
+                      [(3, H, S) for S in (1, 300, 3000) for H in range(1, 120)]):
+            last = 0, None
+            for B, H, S in sizes:
+                n = need(B, H * G, H, S, D)
+                if last[1] is not None and (B, H, S) >= last[1] and sum(
+                        x != y for x, y in zip((B, H, S), last[1])) == 1:
+                    assert n >= last[0], (B, H, S)
+                last = n, (B, H, S)
+    S, D, bs = 40, 128, 64
+    ws = Workspace()
+    _run(160, G, 1, S, D, bs, workspace=ws)
+    size = ws.buf.numel()
+    for B in (159, 149, 148, 147, 75, 2, 1):
+        o, q, *cache = _run(B, G, 1, S, D, bs, workspace=ws)
+        check_attention(o, q, *cache, bs, [S] * B)
+    assert ws.buf.numel() == size and not ws.buf.any()
+
+
 def test_streams_side_by_side():
     """Calls on several streams at once, each with the workspace of its stream."""
     sets = []
