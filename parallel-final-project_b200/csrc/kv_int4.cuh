@@ -422,9 +422,10 @@ __device__ __forceinline__ float inv_rms_exact(const float (&a)[8], const float 
     return rsqrt_rounded(s * (1.0 / D) + eps);
 }
 
-// The same in fp32; rows whose squares leave fp32's range take the fp64 way.
+// The same in fp32; rows whose squares leave fp32's range take the fp64 way, each for itself: a row's
+// bits depend neither on the rows beside it nor on what stands where a row does not exist.
 template <int D>
-__device__ __forceinline__ float inv_rms(const float (&a)[8], const float (&b)[8], double eps) {
+__device__ __forceinline__ float inv_rms(const float (&a)[8], const float (&b)[8], double eps, bool exists) {
     float s = 0.0f, t = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -434,8 +435,13 @@ __device__ __forceinline__ float inv_rms(const float (&a)[8], const float (&b)[8
     s += t;
 #pragma unroll
     for (int off = 1; off < D / 16; off <<= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    if (__any_sync(0xffffffffu, !(s > 1e-30f && s < 1e38f))) return inv_rms_exact<D>(a, b, eps);
-    return __frsqrt_rn(fmaf(s, 1.0f / D, static_cast<float>(eps)));
+    const bool outside = exists && !(s > 1e-30f && s < 1e38f);
+    float inv = __frsqrt_rn(fmaf(s, 1.0f / D, static_cast<float>(eps)));
+    if (__any_sync(0xffffffffu, outside)) {  // all lanes, for the shuffles
+        const float wide = inv_rms_exact<D>(a, b, eps);
+        if (outside) inv = wide;
+    }
+    return inv;
 }
 
 // (p cos - q sin, q cos + p sin), every operation rounded by itself (EXACT) or with FMAs
@@ -652,7 +658,7 @@ __global__ void __launch_bounds__(kInt4Threads, kRopeCtas) qk_norm_rope_kernel(c
         const bool store = h < (kind == 0 ? a.Hq : a.Hkv);
         cp_async_wait<kRopeDepth - 1>();
         uint4(*slot)[32] = mine[(s - s0) % kRopeDepth];
-        float f0[8], f1[8];  // of heads that do not exist: whatever the slot held, stored nowhere
+        float f0[8], f1[8];  // of heads that do not exist: whatever the slot held; nothing comes of it
         unpack8<BF16>(slot[0][lane], f0);
         unpack8<BF16>(slot[1][lane], f1);
         if (kind != 2) {
@@ -667,7 +673,7 @@ __global__ void __launch_bounds__(kInt4Threads, kRopeCtas) qk_norm_rope_kernel(c
                     unpack8<BF16>(reinterpret_cast<const uint4*>(w)[pair1], w1);
                 }
             }
-            const float inv = APPEND ? inv_rms_exact<D>(f0, f1, a.eps) : inv_rms<D>(f0, f1, a.eps);
+            const float inv = APPEND ? inv_rms_exact<D>(f0, f1, a.eps) : inv_rms<D>(f0, f1, a.eps, store);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 f0[j] = __fmul_rn(__fmul_rn(f0[j], inv), w0[j]);
