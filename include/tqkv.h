@@ -350,7 +350,7 @@ tqkv_status tqkv_decode_int8_noalloc(const void* q,
 /* The KV cache in 4 bits (no counterpart in the reference, whose cache has 8).
  *
  * Per row and per block of `block_size` elements, in fp32 with IEEE rounding:
- *   zero = fp16(min x), scale = fp16((max x - min x) * (1 / 15 in fp32)),
+ *   zero = fp16(min x), scale = fp16((max x - min x) / 15),
  *   code = round_half_even((x - zero) / scale) clamped to [0, 15], 0 if scale
  *   is 0; the value read back is code * scale + zero.
  * A block whose scale or zero is not finite (NaN, an infinity or a value
