@@ -31,7 +31,10 @@
 // sums of codes 0..15 would grow with the length while O does not, and what
 // the tensor core cuts off each sum, and p's rounding, would grow with them.
 // K's zero terms are a product as well: a column of zeros times the blocks'
-// sums of q in two fp16 words.
+// sums of q in two fp16 words, 2^14 above the codes' unit, so that they hold all
+// that fp32 does: keys with a large mean have zeros far above their scales (with
+// the words in the codes' unit, off by 2^-15 of the largest |q|, zeros of 4000 moved O
+// by 1 to 4 %).  Up to four more instructions a 16 rows: B1 H32 S65536 52.3 -> 52.5 us.
 //
 // Range.  p * scale must stay inside fp16 whatever the caches hold: the
 // operand is 2^(score - M - e + 11) * scale with M within 2^4 of the largest
@@ -506,6 +509,9 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
         const int nq = left_heads < C::kQ ? left_heads : C::kQ;
 
         // ---- q of the unit as the products' right operands
+        // the scores' unit: the zero terms', 2^-10, where raising the blocks' scales takes fewer
+        // instructions than lowering the zero terms, else the codes', 2^-24
+        constexpr bool kZeroUnit = C::kNS <= 2 * NT;
         uint32_t qf[NT][C::kSub][2][2], qz[NT];
         float sc[NT][2];
 #pragma unroll
@@ -542,20 +548,20 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
                 qf[t][b][1][0] = pack2<false>(f[b][1] * 0.0625f, f[b][5] * 0.0625f);
                 qf[t][b][1][1] = pack2<false>(f[b][3] * 0.0625f, f[b][7] * 0.0625f);
             }
-            // block c's sum (below 2^22) * 2^-24, the codes' unit, as a sum of two fp16, against
-            // its zero twice: off by 2^-25, or 2^-15 of the largest |q|
+            // block c's sum (below 2^22) * 2^-10 as a sum of two fp16, against its zero twice:
+            // off by 2^-23 of the sum or 2^-25, which is 2^-29 of the largest |q|
             float mine_sum = 0.0f;
 #pragma unroll
             for (int s = 0; s < C::kNS; ++s) {
                 sum[s] += __shfl_xor_sync(0xffffffffu, sum[s], 1);
                 sum[s] += __shfl_xor_sync(0xffffffffu, sum[s], 2);
-                if (c == s) mine_sum = sum[s] * 5.9604644775390625e-08f;
+                if (c == s) mine_sum = sum[s] * 0.0009765625f;
             }
             const float high = __half2float(__float2half_rn(mine_sum));
             qz[t] = pack2<false>(high, mine_sum - high);
             // the scores' columns in this lane are heads 2c and 2c + 1
-            const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23) * 16777216.0f *
-                               a.score_scale;
+            const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23) *
+                               (kZeroUnit ? 1024.0f : 16777216.0f) * a.score_scale;
             sc[t][0] = __shfl_sync(0xffffffffu, down, 8 * c);
             sc[t][1] = __shfl_sync(0xffffffffu, down, 8 * c + 4);
         }
@@ -607,6 +613,10 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) s[t][m][i] = 0.0f;
                     mma_f16(s[t][m], z0, z1, 0u, 0u, qz[t], 0u);
+                    if constexpr (!kZeroUnit) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[t][m][i] *= 6.103515625e-05f;
+                    }
                 }
                 float d[NT][4];
 #pragma unroll
@@ -627,8 +637,9 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
                     }
                     if ((b + 1) % (BS / 32) == 0) {
                         const int blk = b * 32 / BS;
-                        const float a0 = __low2float(*reinterpret_cast<const __half2*>(&q0[blk]));
-                        const float a1 = __low2float(*reinterpret_cast<const __half2*>(&q1[blk]));
+                        const float up = kZeroUnit ? 16384.0f : 1.0f;
+                        const float a0 = __low2float(*reinterpret_cast<const __half2*>(&q0[blk])) * up;
+                        const float a1 = __low2float(*reinterpret_cast<const __half2*>(&q1[blk])) * up;
 #pragma unroll
                         for (int t = 0; t < NT; ++t)
 #pragma unroll
