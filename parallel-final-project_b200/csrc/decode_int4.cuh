@@ -19,9 +19,10 @@
 // 2^-20: one AND yields two operands, products with them are exact, sums are
 // fp32.  q is scaled by a power of two per head (exact) and by 2^-4 where it
 // meets the second kind.
-//   score_t = sum_blocks scale_t (codes . q) + zero_t (sum of q over the block)
+//   score_t = sum_blocks (scale_t u) (codes . q) + zero_t (sum of u q over the block)
 //   O       = [ sum_t (p_t scale_t) codes_t + sum_t p_t zero_t ] / sum_t p_t
-// The block scale is applied to the score in fp32; for V it is multiplied into
+// with u = log2(e) / sqrt(D): a score is then a power of two times its logarithm
+// of two.  The block scale is applied to the score in fp32; for V it is multiplied into
 // p in fp32 before p is rounded to fp16 as the product's operand (relative
 // error 2^-11 a token, like the 16-bit P of any tensor-core attention).  The
 // zero sums stay in fp32.
@@ -39,7 +40,11 @@
 // Range.  p * scale must stay inside fp16 whatever the caches hold: the
 // operand is 2^(score - M - e + 11) * scale with M within 2^4 of the largest
 // score so far and 2^e above the largest scale, so it is below 2^15, and
-// tokens 2^-24 of the largest keep all their bits.
+// tokens 2^-24 of the largest keep all their bits.  fp32 holds M + e - 11 to 1 / 4 up
+// to 2^22.  Scores that fp16's q and K reach (2^38) leave no place for e there, and
+// weights 2^(score - M') with another M' than meant would leave the operand's range
+// (q = K = 1000 gave NaN); beyond 2^22 the reference is therefore M itself, the
+// largest score, whose weight is 1 then: exactly, as the score's unit is a power of two.
 //
 // Copies.  Over many tokens O is a sum of terms that cancel, and the operands'
 // rounding shows beside fp16's own: 3.2e-4 of O in the mean, where an O rounded
@@ -120,7 +125,7 @@ struct Int4DecodeArgs {
     int B, Hq, Hkv, group, slices, S;
     int rec_rows;               // query heads a record holds: min(group, 8 * NT)
     int stride;                 // columns of the products from a head to its next copy: 1, 2, 4; 8 without
-    float score_scale;          // log2(e) / sqrt(D)
+    float score_scale;          // u = log2(e) / sqrt(D)
 };
 
 // A unit that a warp's run cuts: its first granule (-1: none, -2: the warp has
@@ -509,9 +514,11 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
         const int nq = left_heads < C::kQ ? left_heads : C::kQ;
 
         // ---- q of the unit as the products' right operands
-        // the scores' unit: the zero terms', 2^-10, where raising the blocks' scales takes fewer
-        // instructions than lowering the zero terms, else the codes', 2^-24
-        constexpr bool kZeroUnit = C::kNS <= 2 * NT;
+        // u, and from the codes' 2^-24 to the sums' 2^-10: a factor of the blocks' scales, or of the
+        // score, its zero terms lowered first, where that is fewer products (32 ragged sequences,
+        // blocks of 32: 28.4 us by the first way, 27.9 by the second)
+        constexpr bool kScaleBlocks = C::kNS <= 2 * NT;
+        const float unit = 16384.0f * a.score_scale;
         uint32_t qf[NT][C::kSub][2][2], qz[NT];
         float sc[NT][2];
 #pragma unroll
@@ -548,26 +555,26 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
                 qf[t][b][1][0] = pack2<false>(f[b][1] * 0.0625f, f[b][5] * 0.0625f);
                 qf[t][b][1][1] = pack2<false>(f[b][3] * 0.0625f, f[b][7] * 0.0625f);
             }
-            // block c's sum (below 2^22) * 2^-10 as a sum of two fp16, against its zero twice:
-            // off by 2^-23 of the sum or 2^-25, which is 2^-29 of the largest |q|
+            // block c's sum (below 2^22) * 2^-10 (and u) as a sum of two fp16, against its zero twice:
+            // off by 2^-23 of it or 2^-25, which is 2^-26 of the largest |q| at most
             float mine_sum = 0.0f;
 #pragma unroll
             for (int s = 0; s < C::kNS; ++s) {
                 sum[s] += __shfl_xor_sync(0xffffffffu, sum[s], 1);
                 sum[s] += __shfl_xor_sync(0xffffffffu, sum[s], 2);
-                if (c == s) mine_sum = sum[s] * 0.0009765625f;
+                if (c == s) mine_sum = sum[s] * 0.0009765625f * (kScaleBlocks ? a.score_scale : 1.0f);
             }
             const float high = __half2float(__float2half_rn(mine_sum));
             qz[t] = pack2<false>(high, mine_sum - high);
             // the scores' columns in this lane are heads 2c and 2c + 1
-            const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23) *
-                               (kZeroUnit ? 1024.0f : 16777216.0f) * a.score_scale;
+            const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23) * 1024.0f;
             sc[t][0] = __shfl_sync(0xffffffffu, down, 8 * c);
             sc[t][1] = __shfl_sync(0xffffffffu, down, 8 * c + 4);
         }
 
-        // R = M + e - 11, M the largest score (base 2) so far, or up to 4 less; `limit`: the raw
-        // score beyond which R has to move
+        // R = M + e - 11, M the largest score (base 2) so far, or up to 4 less, and `limit` the
+        // raw score beyond which R has to move, M + 4; far from 0 R = M, the largest, and `limit` too
+        constexpr float kFar = 4194304.0f;
         float acc[NT][C::kSub][2][4], zsum[NT][C::kNS][2], R[NT][2], limit[NT][2], l[NT][2];
         float scale_top = 0.0f;  // 2^e
 #pragma unroll
@@ -613,10 +620,12 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) s[t][m][i] = 0.0f;
                     mma_f16(s[t][m], z0, z1, 0u, 0u, qz[t], 0u);
-                    if constexpr (!kZeroUnit) {
+                }
+                if constexpr (!kScaleBlocks) {
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) s[t][m][i] *= 6.103515625e-05f;
-                    }
                 }
                 float d[NT][4];
 #pragma unroll
@@ -637,15 +646,21 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
                     }
                     if ((b + 1) % (BS / 32) == 0) {
                         const int blk = b * 32 / BS;
-                        const float up = kZeroUnit ? 16384.0f : 1.0f;
-                        const float a0 = __low2float(*reinterpret_cast<const __half2*>(&q0[blk])) * up;
-                        const float a1 = __low2float(*reinterpret_cast<const __half2*>(&q1[blk])) * up;
+                        float a0 = __low2float(*reinterpret_cast<const __half2*>(&q0[blk]));
+                        float a1 = __low2float(*reinterpret_cast<const __half2*>(&q1[blk]));
+                        if constexpr (kScaleBlocks) a0 *= unit, a1 *= unit;
 #pragma unroll
                         for (int t = 0; t < NT; ++t)
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
                                 s[t][m][i] = fmaf(d[t][i], i < 2 ? a0 : a1, s[t][m][i]);
                     }
+                }
+                if constexpr (!kScaleBlocks) {
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[t][m][i] *= unit;
                 }
             }
             if (left < C::kTile) {
@@ -688,7 +703,6 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
                 for (int off = 4; off < 32; off <<= 1)
                     bigf = fmaxf(bigf, __shfl_xor_sync(0xffffffffu, bigf, off));
                 // the power of two above, and its exponent
-                const float e_old = static_cast<float>(static_cast<int>(__float_as_uint(scale_top) >> 23) - 127);
                 scale_top = fmaxf(scale_top,
                                   __uint_as_float((__float_as_uint(bigf) + 0x00800000u) & 0x7f800000u));
                 const float e = static_cast<float>(static_cast<int>(__float_as_uint(scale_top) >> 23) - 127);
@@ -702,9 +716,10 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
                             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
                         // copy i of a head: i / copies higher
                         const float up = NT == 1 ? 0.125f * static_cast<float>((2 * c + j) & -a.stride) : 0.0f;
-                        const float m = fmaxf(x, R[t][j] + (11.0f - e_old - up));
-                        const float r = m + (e - 11.0f + up);
-                        limit[t][j] = (m + 4.0f) / sc[t][j];
+                        const float y = limit[t][j] * sc[t][j];
+                        const float m = fmaxf(x, fabsf(y) > kFar ? y : y - 4.0f);
+                        const float r = fabsf(m) > kFar ? m : m + (e - 11.0f + up);
+                        limit[t][j] = (fabsf(m) > kFar ? m : m + 4.0f) / sc[t][j];
                         const float f = r == R[t][j] ? 1.0f : fast_exp2(R[t][j] - r);
                         R[t][j] = r;
                         l[t][j] *= f;
