@@ -535,9 +535,9 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
             // 2^e with max |q| * 2^e in [2^14, 2^15): exact in fp16, also over 16, down
-            // to 2^-24 of the largest element
+            // to 2^-24 of the largest element; an infinite one stays so
             int e = 141 - static_cast<int>(__float_as_uint(amax) >> 23);
-            e = amax == 0.0f || amax > 3.0e38f ? 0 : e > 100 ? 100 : e < -100 ? -100 : e;
+            e = amax == 0.0f ? 0 : e > 100 ? 100 : e;
             const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
             float sum[C::kNS];
 #pragma unroll
@@ -566,8 +566,11 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
             }
             const float high = __half2float(__float2half_rn(mine_sum));
             qz[t] = pack2<false>(high, mine_sum - high);
-            // the scores' columns in this lane are heads 2c and 2c + 1
-            const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23) * 1024.0f;
+            // the scores' columns in this lane are heads 2c and 2c + 1.  2^(10 - e), or 2^80: sums
+            // differ by 2^-60 if at all (codes * 2^-24, q and scales of 2^-24 each, the unit's 2^12 and
+            // more), so that all but the largest then weigh nothing either way, and are below 2^34:
+            // no score overflows
+            const float down = fminf(__uint_as_float(static_cast<uint32_t>(127 - e) << 23) * 1024.0f, 0x1p80f);
             sc[t][0] = __shfl_sync(0xffffffffu, down, 8 * c);
             sc[t][1] = __shfl_sync(0xffffffffu, down, 8 * c + 4);
         }

@@ -1,5 +1,5 @@
-"""Scores of the 4-bit decode where they are hard to hold: keys with a large zero, and scores far beyond
-the weights' range."""
+"""Scores of the 4-bit decode where they are hard to hold: keys with a large zero, scores far beyond
+the weights' range, and queries up to the end of bf16's."""
 import numpy as np
 import pytest
 import torch
@@ -119,8 +119,20 @@ def test_scores_far_beyond_the_weights_range(S, peaks, D, bs, qmul, kmul, dtype)
     assert torch.isfinite(o).all()
 
 
+@pytest.mark.parametrize("D,bs", VALID)
+@pytest.mark.parametrize("qmul", [2.0 ** 90, 8e34, 1e38, 3.38e38])
+@pytest.mark.parametrize("kmul", [1e-6, 1.0, 60000.0])
+def test_bf16_queries_up_to_the_end_of_their_range(D, bs, qmul, kmul):
+    S, peaks = 300, [3, 299, 128]
+    (kq, ks), pattern = _keys(S, D, bs, D, kmul, peaks)
+    g = torch.Generator(device="cuda").manual_seed(S)
+    vq, vs = tqkv.kv_compress_int4(torch.randn((1, 1, S, D), generator=g, device="cuda").half(), bs)
+    q = torch.from_numpy(pattern * qmul)[None].to(BF16).cuda()
+    _one_hot(q, kq, ks, vq, vs, bs, BF16, 2.0 ** -7)
+
+
 @pytest.mark.parametrize("D,bs", [(64, 32), (128, 128)])
-@pytest.mark.parametrize("qmul,kmul", [(1.0, 1.0), (60000.0, 60000.0), (1e-30, 1.0)])
+@pytest.mark.parametrize("qmul,kmul", [(1.0, 1.0), (60000.0, 60000.0), (1e-30, 1.0), (3e38, 1.0), (3e38, 60000.0)])
 def test_equal_scores_of_any_size_share_the_weight(D, bs, qmul, kmul):
     """All keys alike, in one piece and in many: O is the mean of V."""
     for S in (70, 4000):
