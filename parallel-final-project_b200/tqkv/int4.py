@@ -214,8 +214,7 @@ def _workspace(ws: Optional[Workspace], index: int, handle: int, key):
     if need == 0:
         return None, 0
     if ws is not None:
-        if ws.device.index not in (None, index):
-            raise ValueError(f"workspace is on {ws.device}, tensors are on cuda:{index}")
+        ws.check_device(index)
         if ws.buf is not None and ws.buf.numel() >= need:
             return ws.buf.data_ptr(), ws.buf.numel()
     if torch.cuda.is_current_stream_capturing():

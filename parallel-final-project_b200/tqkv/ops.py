@@ -194,6 +194,12 @@ class Workspace:
         self.buf: Optional[torch.Tensor] = None
         self._retired: list = []
 
+    def check_device(self, index: int) -> None:
+        """Refuse a call whose tensors are not where the buffer is, or, before there is one, will be."""
+        at = self.device.index if self.buf is None else self.buf.get_device()
+        if at is not None and at != index:
+            raise ValueError(f"workspace is on cuda:{at}, tensors are on cuda:{index}")
+
     def get(self, nbytes: int, stream=None) -> Tuple[Optional[int], int]:
         if nbytes == 0:
             return None, 0
@@ -213,6 +219,7 @@ _default_ws: dict = {}
 
 def _workspace(ws: Optional[Workspace], device: torch.device) -> Workspace:
     if ws is not None:
+        ws.check_device(device.index)
         return ws
     key = (device.index, torch.cuda.current_stream(device).cuda_stream)
     if key not in _default_ws:
