@@ -215,8 +215,9 @@ def _workspace(ws: Optional[Workspace], index: int, handle: int, key):
         return None, 0
     if ws is not None:
         ws.check_device(index)
-        if ws.buf is not None and ws.buf.numel() >= need:
-            return ws.buf.data_ptr(), ws.buf.numel()
+        buf = ws.buf
+        if buf is not None and buf.numel() >= need:
+            return buf.data_ptr(), buf.numel()
     if torch.cuda.is_current_stream_capturing():
         if ws is not None:
             raise ValueError("a Workspace cannot grow while a graph is captured: call once before "
@@ -229,7 +230,7 @@ def _workspace(ws: Optional[Workspace], index: int, handle: int, key):
     if ws is None:
         ws = _default_ws.get((index, handle))
         if ws is None:
-            ws = _default_ws[(index, handle)] = Workspace(torch.device("cuda", index))
+            ws = _default_ws.setdefault((index, handle), Workspace(torch.device("cuda", index)))
     return ws.get(need)
 
 

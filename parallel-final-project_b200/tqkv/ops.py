@@ -15,6 +15,7 @@ sm_100a kernels.  Errors raise TqkvError.
 from __future__ import annotations
 
 import ctypes
+import threading
 from typing import Optional, Tuple
 
 import torch
@@ -193,6 +194,7 @@ class Workspace:
             else torch.device(device)
         self.buf: Optional[torch.Tensor] = None
         self._retired: list = []
+        self._growing = threading.Lock()
 
     def check_device(self, index: int) -> None:
         """Refuse a call whose tensors are not where the buffer is, or, before there is one, will be."""
@@ -203,15 +205,20 @@ class Workspace:
     def get(self, nbytes: int, stream=None) -> Tuple[Optional[int], int]:
         if nbytes == 0:
             return None, 0
-        if self.buf is None or self.buf.numel() < nbytes:
-            size = nbytes if self.buf is None else max(nbytes, 2 * self.buf.numel())
-            if self.buf is not None:
-                self._retired.append(self.buf)
-            self.buf = torch.empty(size, dtype=torch.uint8, device=self.device)
-            lib = load()
-            check("tqkv_workspace_init", lib.tqkv_workspace_init(
-                self.buf.data_ptr(), size, _stream_handle(stream)))
-        return self.buf.data_ptr(), self.buf.numel()
+        buf = self.buf
+        if buf is None or buf.numel() < nbytes:
+            # another thread of the same stream sees the new buffer once its zeroing is enqueued
+            with self._growing:
+                buf = self.buf
+                if buf is None or buf.numel() < nbytes:
+                    size = nbytes if buf is None else max(nbytes, 2 * buf.numel())
+                    new = torch.empty(size, dtype=torch.uint8, device=self.device)
+                    check("tqkv_workspace_init", load().tqkv_workspace_init(
+                        new.data_ptr(), size, _stream_handle(stream)))
+                    if buf is not None:
+                        self._retired.append(buf)
+                    self.buf = buf = new
+        return buf.data_ptr(), buf.numel()
 
 
 _default_ws: dict = {}
@@ -222,9 +229,8 @@ def _workspace(ws: Optional[Workspace], device: torch.device) -> Workspace:
         ws.check_device(device.index)
         return ws
     key = (device.index, torch.cuda.current_stream(device).cuda_stream)
-    if key not in _default_ws:
-        _default_ws[key] = Workspace(device)
-    return _default_ws[key]
+    found = _default_ws.get(key)
+    return _default_ws.setdefault(key, Workspace(device)) if found is None else found
 
 
 def decode_int8(q: torch.Tensor, kq: torch.Tensor, ks: torch.Tensor, vq: torch.Tensor,
