@@ -12,7 +12,8 @@ namespace tqkv {
 
 // Device-wide failure flag (first nonzero code wins).  Written by a kernel
 // whose bounded wait ran out; read and cleared by tqkv_read_device_error().
-// The library keeps all device code in one translation unit, which owns it.
+// Each translation unit has its own; all kernels that wait on a barrier or a flag are
+// in tqkv_capi.cu, whose flag is the one that is read.
 static __device__ unsigned int g_device_error = 0;
 
 enum DeviceErrorCode : unsigned int {

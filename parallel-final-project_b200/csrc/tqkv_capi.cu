@@ -1,8 +1,9 @@
 // tqkv_capi.cu — kernel instantiations, launch planning, the per-stream
 // workspace cache and the extern "C" ABI declared in include/tqkv.h.
 //
-// Everything device-side lives in this one translation unit (no relocatable
-// device code), so the device error flag of device_common.cuh is this TU's.
+// Every kernel that waits lives in this translation unit (no relocatable device
+// code), so the device error flag of device_common.cuh is this TU's; the 4-bit
+// kernels (tqkv_int4.cu) wait for nothing but their own copies and record none.
 
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -701,10 +702,7 @@ tqkv_status tqkv_read_device_error(uint32_t* code_out) {
     const unsigned int zero = 0;
     e = cudaMemcpyToSymbol(tqkv::g_device_error, &zero, sizeof(zero));
     if (e != cudaSuccess) return tqkv::from_cuda(e);
-    unsigned int int4 = 0;  // the 4-bit kernels' flag
-    e = tqkv::take_int4_device_error(&int4);
-    if (e != cudaSuccess) return tqkv::from_cuda(e);
-    *code_out = v != 0 ? v : int4;
+    *code_out = v;
     return TQKV_OK;
 }
 

@@ -20,14 +20,6 @@
 
 namespace tqkv {
 
-// This file's copy of the device error flag (device_common.cuh).
-cudaError_t take_int4_device_error(unsigned int* code) {
-    cudaError_t e = cudaMemcpyFromSymbol(code, g_device_error, sizeof(*code));
-    if (e != cudaSuccess || *code == 0) return e;
-    const unsigned int zero = 0;
-    return cudaMemcpyToSymbol(g_device_error, &zero, sizeof(zero));
-}
-
 namespace {
 
 constexpr int kMaxDevices = 64;
@@ -70,13 +62,11 @@ unsigned rows_grid(long long rows, int unroll) {
     return static_cast<unsigned>((rows + per - 1) / per);
 }
 
-tqkv_status make_rows(Int4Rows& g, int B, int H, int T, int D, int S_cap, const int32_t* starts,
-                      int t0) {
+tqkv_status make_rows(Int4Rows& g, int B, int H, int T, int S_cap, const int32_t* starts, int t0) {
     if (B <= 0 || H <= 0 || T <= 0 || S_cap <= 0 || T > S_cap) return TQKV_ERR_INVALID_SIZE;
     if (!starts && (t0 < 0 || static_cast<long long>(t0) + T > S_cap)) return TQKV_ERR_INVALID_SIZE;
     const long long BH = static_cast<long long>(B) * H;
     if (BH > INT_MAX / T) return TQKV_ERR_INVALID_SIZE;
-    (void)D;
     g.rows = static_cast<uint32_t>(BH * T);
     g.T = FastDiv(static_cast<uint32_t>(T));
     g.H = FastDiv(static_cast<uint32_t>(H));
@@ -95,7 +85,7 @@ struct DecodePlan4 {
     long long counted;          // granules that they and the units count for
 };
 
-DecodePlan4 plan_int4(int B, int Hq, int Hkv, int S, int D) {
+DecodePlan4 plan_int4(int B, int Hq, int Hkv, int S) {
     DecodePlan4 p{};
     const int group = Hq / Hkv;
     p.nt = group > 8 ? 2 : 1;
@@ -163,7 +153,7 @@ tqkv_status tqkv_kv_append_int4(const void* x, const long long* x_strides, uint8
                                 int D, int block_size, int S_cap, int dtype, cudaStream_t stream) {
     if (!is_supported_int8(D, block_size) || !is_16bit(dtype)) return TQKV_ERR_UNSUPPORTED;
     Int4Rows g;
-    const tqkv_status st = make_rows(g, B, H, T, D, S_cap, starts, t0);
+    const tqkv_status st = make_rows(g, B, H, T, S_cap, starts, t0);
     if (st != TQKV_OK) return st;
     if (!x || !cache_q || !cache_s) return TQKV_ERR_NULL;
     if (!aligned(x, 16) || !aligned(cache_q, 16) || !aligned(cache_s, 16) ||
@@ -193,7 +183,7 @@ tqkv_status tqkv_kv_reconstruct_int4(const uint8_t* cache_q, const void* cache_s
                                      int block_size, int S_cap, int dtype, cudaStream_t stream) {
     if (!is_supported_int8(D, block_size) || !is_16bit(dtype)) return TQKV_ERR_UNSUPPORTED;
     Int4Rows g;
-    const tqkv_status st = make_rows(g, B, H, T, D, S_cap, starts, t0);
+    const tqkv_status st = make_rows(g, B, H, T, S_cap, starts, t0);
     if (st != TQKV_OK) return st;
     if (!cache_q || !cache_s || !y) return TQKV_ERR_NULL;
     if (!aligned(cache_q, 16) || !aligned(cache_s, 16) || !aligned(y, 16) || !aligned(starts, 4))
@@ -213,7 +203,7 @@ size_t tqkv_decode_int4_workspace_bytes(int B, int H_q, int H_kv, int S, int D) 
         return 0;
     int dev = 0, sms = 0;
     if (current_sms(&dev, &sms) != cudaSuccess) return 0;
-    const DecodePlan4 p = plan_int4(B, H_q, H_kv, S, D);
+    const DecodePlan4 p = plan_int4(B, H_q, H_kv, S);
     return int4_workspace(p, D, sms);
 }
 
@@ -245,7 +235,7 @@ tqkv_status tqkv_decode_int4(const void* q, const uint8_t* kq, const void* ks, c
     a.group = H_q / H_kv;
     a.S = S;
     a.score_scale = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(D)));
-    const DecodePlan4 p = plan_int4(B, H_q, H_kv, S, D);
+    const DecodePlan4 p = plan_int4(B, H_q, H_kv, S);
     if (p.granules + p.units * kUnitCost > INT_MAX) return TQKV_ERR_INVALID_SIZE;
     a.slices = p.slices;
     a.rec_rows = p.rec_rows;

@@ -19,10 +19,6 @@ tqkv_status from_cuda(cudaError_t err);
 
 bool is_supported_int8(int D, int block_size);
 
-// Reads and clears the device error flag of the 4-bit kernels, which are a
-// translation unit of their own (tqkv_int4.cu).
-cudaError_t take_int4_device_error(unsigned int* code);
-
 // Kernel launches with all checks done by the caller except alignment.
 // T > 0: the rows are T new tokens per head, written to rows [t0, t0 + T) of a
 // cache holding S_cap rows per head; T <= 0: whole tensors, in place.
