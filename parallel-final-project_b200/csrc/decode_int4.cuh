@@ -24,8 +24,8 @@
 // with u = log2(e) / sqrt(D): a score is then a power of two times its logarithm
 // of two.  The block scale is applied to the score in fp32; for V it is multiplied into
 // p in fp32 before p is rounded to fp16 as the product's operand (relative
-// error 2^-11 a token, like the 16-bit P of any tensor-core attention).  The
-// zero sums stay in fp32.
+// error 2^-11 a token, like the 16-bit P of any tensor-core attention; Copies and
+// Rests, below, take it out of fp16 outputs).  The zero sums stay in fp32.
 //
 // V's codes enter as code - 8 for even tokens and code - 7 for odd ones (one
 // packed fp16 subtraction, exact) beside zero + 8 scale and zero + 7 scale:
@@ -55,6 +55,12 @@
 // takes as long as before; the mean costs a piece 0.3 to 0.8 us (B1 H32 S65536
 // 51.9 -> 52.3 us, 512 heads of one row 4.3 -> 4.9 us).  Remainders of the weights
 // in the idle columns gave 2.0e-4, but 55.3 us.  bf16's rounding covers all of it.
+//
+// Rests.  fp16 groups of 5 and more have no column to spare, and O was 1.5 to 1.6 times as
+// far off as one rounded once.  What rounding takes off the operand is a second
+// operand there, rounded to fp16 itself (2^-22): 3.2e-4 -> 2.1e-4, which is O's own
+// rounding.  32 ragged sequences, 64/8 heads of 128: 26.6 -> 27.3 us (block 128), 28.7 ->
+// 31.8 (block 32); 64/4 heads 26.4 -> 29.8; B4 64/8 heads S65536 54 -> 65.
 //
 // Work split.  Units are (sequence, KV head, slice of 8 * NT query heads); a
 // unit has ceil(length / 16) granules, and counts for six more, about what
@@ -135,7 +141,8 @@ struct alignas(16) CutUnit {
     int start, end, row, nq;
 };
 
-template <int D, int BS, int NT>
+// REST: weights as two fp16 operands, for fp16 outputs of groups without idle columns
+template <int D, int BS, int NT, bool REST>
 struct I4Cfg {
     static constexpr int kRow = D / 2;            // bytes of codes a row
     static constexpr int kSub = D / 32;           // 32-element groups = words per lane chunk
@@ -153,8 +160,10 @@ struct I4Cfg {
     // Warps of a CTA, one CTA an SM: 12 leave each 168 registers, 8 leave 255.  12
     // hide more latency (B1 H32 S65536, block 128: 51.9 us, 57.2 with 8 and with 16)
     // unless two sets of accumulators (NT = 2) or four blocks a row spill (B1 32/8
-    // heads S65536, block 32: 25.8 us with 12, 24.0 with 8).
-    static constexpr int kWarps = NT == 2 || kNS == 4 ? 8 : 12;
+    // heads S65536, block 32: 25.8 us with 12, 24.0 with 8), or the weights' rests need
+    // the registers (32 ragged sequences, 64/8 heads of 128, block 64: 33.0 and 29.3; of 64: 22.4
+    // and 23.2).
+    static constexpr int kWarps = NT == 2 || kNS == 4 || (REST && D == 128) ? 8 : 12;
     static_assert(kWarps >= kI4MinWarps, "the workspace holds a record pair for every CTA");
     // bytes of the states of `rows` query heads
     __host__ __device__ static constexpr int state(int rows) { return rows * kRecStride * 4; }
@@ -281,14 +290,14 @@ struct UnitWalk {
     }
 };
 
-static_assert(I4Cfg<128, 32, 1>::smem_bytes(8) <= 227 * 1024 &&
-                  I4Cfg<128, 32, 2>::smem_bytes(16) <= 227 * 1024,
+static_assert(I4Cfg<128, 32, 1, false>::smem_bytes(8) <= 227 * 1024 &&
+                  I4Cfg<128, 32, 2, false>::smem_bytes(16) <= 227 * 1024,
               "the stages and the states of any group fit");
 
-template <int D, int BS, int NT>
-__global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
+template <int D, int BS, int NT, bool REST>
+__global__ void __launch_bounds__(I4Cfg<D, BS, NT, REST>::kWarps * 32, 1)
     decode_int4_kernel(const Int4DecodeArgs a, int bf16) {
-    using C = I4Cfg<D, BS, NT>;
+    using C = I4Cfg<D, BS, NT, REST>;
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int nw = C::kWarps;
@@ -783,11 +792,20 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
                     float2 vb = __half22float2(*reinterpret_cast<const __half2*>(&q1[k]));
                     va.y = fmaf(va.x, middle, va.y);
                     vb.y = fmaf(vb.x, middle, vb.y);
-                    uint32_t bw[NT][2];
+                    uint32_t bw[NT][2], rest[NT][2];  // p * scale, and what its rounding took off
 #pragma unroll
                     for (int t = 0; t < NT; ++t) {
-                        bw[t][0] = movmatrix(pack2<false>(p[t][0] * va.x, p[t][1] * va.x));
-                        bw[t][1] = movmatrix(pack2<false>(p[t][2] * vb.x, p[t][3] * vb.x));
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            const float scale = r == 0 ? va.x : vb.x;
+                            const float w0 = p[t][2 * r] * scale, w1 = p[t][2 * r + 1] * scale;
+                            const uint32_t w = pack2<false>(w0, w1);
+                            bw[t][r] = movmatrix(w);
+                            if constexpr (REST) {
+                                const float2 have = __half22float2(*reinterpret_cast<const __half2*>(&w));
+                                rest[t][r] = movmatrix(pack2<false>(w0 - have.x, w1 - have.y));
+                            }
+                        }
                         zsum[t][k][0] = fmaf(p[t][0], va.y, fmaf(p[t][2], vb.y, zsum[t][k][0]));
                         zsum[t][k][1] = fmaf(p[t][1], va.y, fmaf(p[t][3], vb.y, zsum[t][k][1]));
                     }
@@ -803,6 +821,10 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
                         for (int t = 0; t < NT; ++t) {
                             mma_f16(acc[t][b][0], a0, a1, a2, a3, bw[t][0], bw[t][1]);
                             mma_f16(acc[t][b][1], c0, c1, c2, c3, bw[t][0], bw[t][1]);
+                            if constexpr (REST) {
+                                mma_f16(acc[t][b][0], a0, a1, a2, a3, rest[t][0], rest[t][1]);
+                                mma_f16(acc[t][b][1], c0, c1, c2, c3, rest[t][0], rest[t][1]);
+                            }
                         }
                     }
                 }
@@ -818,7 +840,7 @@ __global__ void __launch_bounds__(I4Cfg<D, BS, NT>::kWarps * 32, 1)
         }
 
         // ---- the mean of a head's copies, at the first one's reference
-        if (NT == 1 && a.stride < 8) {
+        if (NT == 1 && !REST && a.stride < 8) {
             const bool one = a.stride == 1;
             const int first = (lane & ~3) | (c & ((a.stride >> 1) - (one ? 0 : 1)));
             const float base0 = __shfl_sync(0xffffffffu, R[0][0], first);

@@ -116,14 +116,14 @@ size_t int4_workspace(const DecodePlan4& p, int D, int sms) {
     return int4_counters(grid) + static_cast<size_t>(grid) * 2 * p.rec_rows * (D + 4) * sizeof(float);
 }
 
-template <int D, int BS, int NT>
+template <int D, int BS, int NT, bool REST>
 tqkv_status decode_int4_impl(Int4DecodeArgs a, const DecodePlan4& p, int bf16, void* workspace,
                              size_t workspace_bytes, cudaStream_t stream) {
-    using C = I4Cfg<D, BS, NT>;
+    using C = I4Cfg<D, BS, NT, REST>;
     int dev = 0, sms = 0;
     cudaError_t e = current_sms(&dev, &sms);
     if (e != cudaSuccess) return from_cuda(e);
-    auto fn = decode_int4_kernel<D, BS, NT>;
+    auto fn = decode_int4_kernel<D, BS, NT, REST>;
     constexpr int kSmem = 227 * 1024;
     static std::atomic<bool> opted[kMaxDevices];
     if (!opted[dev].load(std::memory_order_acquire)) {
@@ -240,11 +240,19 @@ tqkv_status tqkv_decode_int4(const void* q, const uint8_t* kq, const void* ks, c
     a.slices = p.slices;
     a.rec_rows = p.rec_rows;
     const int bf16 = dtype == TQKV_BF16;
-    a.stride = 8;  // fp16: copies of the heads in the columns that a small group leaves idle
+    a.stride = 8;  // fp16: copies of the heads in the columns that a small group leaves idle, or rests
     while (!bf16 && a.stride / 2 >= a.group) a.stride /= 2;
     return for_shape(D, block_size, [&](auto d, auto bs) {
-        return p.nt == 1 ? decode_int4_impl<d(), bs(), 1>(a, p, bf16, workspace, workspace_bytes, stream)
-                         : decode_int4_impl<d(), bs(), 2>(a, p, bf16, workspace, workspace_bytes, stream);
+        auto run = [&](auto nt, auto rest) {
+            return decode_int4_impl<d(), bs(), nt(), rest()>(a, p, bf16, workspace, workspace_bytes, stream);
+        };
+        using std::integral_constant;
+        using std::bool_constant;
+        if (p.nt == 2)
+            return bf16 ? run(integral_constant<int, 2>{}, bool_constant<false>{})
+                        : run(integral_constant<int, 2>{}, bool_constant<true>{});
+        return bf16 || a.stride < 8 ? run(integral_constant<int, 1>{}, bool_constant<false>{})
+                                    : run(integral_constant<int, 1>{}, bool_constant<true>{});
     });
 }
 
