@@ -35,16 +35,16 @@
 // sums of q in two fp16 words, 2^14 above the codes' unit, so that they hold all
 // that fp32 does: keys with a large mean have zeros far above their scales (with
 // the words in the codes' unit, off by 2^-15 of the largest |q|, zeros of 4000 moved O
-// by 1 to 4 %).  Up to four more instructions a 16 rows: B1 H32 S65536 52.3 -> 52.5 us.
+// by 1 to 4 %).  B1 H32 S65536 52.3 -> 52.5 us.
 //
 // Range.  p * scale must stay inside fp16 whatever the caches hold: the
 // operand is 2^(score - M - e + 11) * scale with M within 2^4 of the largest
 // score so far and 2^e above the largest scale, so it is below 2^15, and
 // tokens 2^-24 of the largest keep all their bits.  fp32 holds M + e - 11 to 1 / 4 up
 // to 2^22.  Scores that fp16's q and K reach (2^38) leave no place for e there, and
-// weights 2^(score - M') with another M' than meant would leave the operand's range
-// (q = K = 1000 gave NaN); beyond 2^22 the reference is therefore M itself, the
-// largest score, whose weight is 1 then: exactly, as the score's unit is a power of two.
+// the weights would leave the operand's range by a rounding of the reference (q = K =
+// 1000 gave NaN); beyond 2^22 the reference is therefore M itself, the largest score,
+// whose weight is 1 then: exactly, as the score's unit is a power of two.
 //
 // Copies.  Over many tokens O is a sum of terms that cancel, and the operands'
 // rounding shows beside fp16's own: 3.2e-4 of O in the mean, where an O rounded
@@ -66,7 +66,8 @@
 // unit has ceil(length / 16) granules, and counts for six more, about what
 // starting and ending it costs (ragged lengths put many short units into one
 // run: 37.3 us without, 30.9 with it for 32 sequences of 1 to 4099 rows and 8 KV
-// heads).  All units' granules, end to end, are cut
+// heads; 3, 6 and 12 are 28.3, 27.6 and 28.5 there, 23.8, 21.9 and 21.9 with heads of
+// 64, 29.6, 26.6 and 26.8 with 16 query heads a KV head).  All units' granules, end to end, are cut
 // into equal runs, one per CTA, and each CTA's run into equal runs, one per
 // warp, whatever the lengths are.  A warp meets at most one unit that began
 // before its run and one that goes on behind it; units that lie within its run
