@@ -198,9 +198,9 @@ class Workspace:
 
     def check_device(self, index: int) -> None:
         """Refuse a call whose tensors are not where the buffer is, or, before there is one, will be."""
-        at = self.device.index if self.buf is None else self.buf.get_device()
-        if at is not None and at != index:
-            raise ValueError(f"workspace is on cuda:{at}, tensors are on cuda:{index}")
+        at = self.device if self.buf is None else self.buf.device
+        if at.type != "cuda" or at.index not in (None, index):
+            raise ValueError(f"workspace is on {at}, tensors are on cuda:{index}")
 
     def get(self, nbytes: int, stream=None) -> Tuple[Optional[int], int]:
         if nbytes == 0:

@@ -41,6 +41,17 @@ def test_a_workspace_for_another_device_is_refused_before_it_has_a_buffer(sizes)
         ops._workspace(ws, torch.device("cuda:1"))
 
 
+def test_a_workspace_in_host_memory_is_refused(sizes):
+    """Its buffer's address would go to a kernel."""
+    ws = ops.Workspace("cpu")
+    for _ in range(2):
+        with pytest.raises(ValueError, match="workspace is on cpu"):
+            int4._workspace(ws, 0, 0, KEY)
+        with pytest.raises(ValueError, match="workspace is on cpu"):
+            ops._workspace(ws, torch.device("cuda:0"))
+        ws.buf = torch.empty(1 << 20, dtype=torch.uint8)
+
+
 def _grow(monkeypatch, init):
     """A Workspace in host memory whose zeroing is `init`."""
     monkeypatch.setattr(ops, "load", lambda: types.SimpleNamespace(tqkv_workspace_init=init))
