@@ -88,9 +88,10 @@ struct DecodePlan4 {
 DecodePlan4 plan_int4(int B, int Hq, int Hkv, int S) {
     DecodePlan4 p{};
     const int group = Hq / Hkv;
-    // 16 heads a pass beyond 8, where two passes of 8 would read the cache twice: 64/4 heads of 128 (bf16,
-    // block 128) at B4 S131072 89.5 us and 96.8 by two passes, 4 x 36/4 of block 64 95 and 115.  Caches
-    // that L2 holds do not need it: 32 ragged sequences of up to 4099 rows 26.6 and 26.4, B1 S32769 39.4 and 20.8.
+    // More than 8 heads share a pass of 16, where two passes of 8 would read the cache twice: B4 S131072
+    // (heads of 128, bf16) takes 89.5 us with 64/4 heads and blocks of 128, 96.8 by two passes, and 95 with
+    // 36/4 and blocks of 64, 115 by two.  A cache that L2 holds does not need it: 64/4 heads, 32 ragged
+    // sequences of up to 4099 rows 26.6 and 26.4, one of 32769 rows 39.4 and 20.8.
     p.nt = group > 8 ? 2 : 1;
     p.rec_rows = group < 8 * p.nt ? group : 8 * p.nt;
     p.slices = (group + 8 * p.nt - 1) / (8 * p.nt);
